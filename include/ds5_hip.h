@@ -517,8 +517,130 @@ typedef struct ds5_paged_decode_args {
 } ds5_paged_decode_args;
 int ds5_hip_paged_decode(ds5_hip_ctx* ctx, const ds5_paged_decode_args* args);
 
+/* A batch over the paged pool (no reference counterpart; the pool, the page
+ * table and its rules are those of ds5_hip_paged_decode). Row r of the batch
+ * is one new token. Sequence b holds the rows starts[b] .. starts[b + 1] - 1,
+ * its newest tokens, and seq_lens[b] tokens in all, those rows included: with
+ * n_b = starts[b + 1] - starts[b], row starts[b] + i is the token at position
+ * seq_lens[b] - n_b + i. A sequence may hold no row; rows that no sequence
+ * holds (behind starts[n_seqs], say) are left as they were in every output.
+ * starts does not decrease. Device-side entries out of range are never
+ * dereferenced and show as NaN: every row of a sequence whose rows leave
+ * [0, n_tokens) or whose length is outside [n_b, max_seq_len], and every row
+ * that needs a page outside [0, n_pages). max_seq_len is a host-side upper
+ * bound of seq_lens. All views 16-byte aligned (starts, seq_lens and page_table
+ * 4-byte), page_size a multiple of 16, head_dim 64 or 128; no allocation. */
+
+/* Appends the batch's k and v to the pool, k normalised and rotated on the way,
+ * and normalises and rotates q for ds5_hip_paged_attention: per head RMSNorm
+ * with q_norm / k_norm (each optional: len 0 leaves that one out), the NeoX
+ * rotation at the row's position, then k and v as f16 into the position's slot
+ * and q into q_out as q_dtype (f32 or f16). The rotation angle, position *
+ * freq_scale * theta^(-2i/head_dim), is worked out and reduced in 64 bits, so it
+ * holds its accuracy at any position; ds5_hip_paged_decode and the contiguous
+ * ops round it to f32 as the reference does, so their k rows agree with these to
+ * that rounding (8e-4 rad at position 16384). q is optional (len 0: k and v
+ * alone). q_out may be q itself when q_dtype is f32; other overlaps of the
+ * outputs with the inputs are ShapeMismatch. A row that shows as NaN (see above)
+ * does so in q_out, and its k and v are not appended. Two rows of one call must
+ * not share a slot. */
+typedef struct ds5_paged_append_args {
+    ds5_buf q;          /* optional f32 [n_tokens, n_q_heads, head_dim] */
+    ds5_buf k;          /* f32 [n_tokens, n_kv_heads, head_dim] */
+    ds5_buf v;          /* f32 [n_tokens, n_kv_heads, head_dim] */
+    ds5_buf q_norm;     /* optional f32 [head_dim] */
+    ds5_buf k_norm;     /* optional f32 [head_dim] */
+    ds5_buf q_out;      /* q_dtype [n_tokens, n_q_heads, head_dim]; unused without q */
+    ds5_buf k_pool;     /* f16 [n_kv_heads, n_pages * page_size, head_dim] */
+    ds5_buf v_pool;
+    ds5_buf page_table; /* i32 [n_seqs, max_pages] */
+    ds5_buf starts;     /* i32 [n_seqs + 1] */
+    ds5_buf seq_lens;   /* i32 [n_seqs], the appended tokens included */
+    uint32_t q_dtype;   /* DS5_DTYPE_F32 or DS5_DTYPE_F16 */
+    uint32_t n_tokens;
+    uint32_t n_seqs;
+    uint32_t n_q_heads;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;
+    uint32_t page_size;
+    uint32_t n_pages;
+    uint32_t max_pages;
+    uint32_t max_seq_len;
+    float eps;
+    float theta;
+    float freq_scale;
+} ds5_paged_append_args;
+int ds5_hip_paged_append(ds5_hip_ctx* ctx, const ds5_paged_append_args* args);
+
+/* Causal GQA attention of the batch's rows over the pool: row r at position p
+ * of its sequence attends positions 0 .. p (which the pool holds already, its own
+ * among them); softmax in f32, out always f32. One call serves single tokens,
+ * prompts and both mixed. f32 q enters the products with 22 significant bits,
+ * f16 q (as ds5_hip_paged_append writes it) as it is; the softmax weights with 22
+ * bits in either case. What a row does not attend never touches it, whatever the
+ * pool holds there (infinities and NaN included). At most DS5_PAGED_MAX_SEQS
+ * sequences; out must not overlap q or the pools. */
+#define DS5_PAGED_MAX_SEQS 1024u
+typedef struct ds5_paged_attention_args {
+    ds5_buf q;          /* q_dtype [n_tokens, n_q_heads, head_dim], normalised and rotated */
+    ds5_buf k_pool;     /* f16 [n_kv_heads, n_pages * page_size, head_dim] */
+    ds5_buf v_pool;
+    ds5_buf page_table; /* i32 [n_seqs, max_pages] */
+    ds5_buf starts;     /* i32 [n_seqs + 1] */
+    ds5_buf seq_lens;   /* i32 [n_seqs] */
+    ds5_buf out;        /* f32 [n_tokens, n_q_heads * head_dim] */
+    uint32_t q_dtype;   /* DS5_DTYPE_F32 or DS5_DTYPE_F16 */
+    uint32_t n_tokens;
+    uint32_t n_seqs;
+    uint32_t n_q_heads;
+    uint32_t n_kv_heads;
+    uint32_t head_dim;
+    uint32_t page_size;
+    uint32_t n_pages;
+    uint32_t max_pages;
+    uint32_t max_seq_len;
+    float scale;
+} ds5_paged_attention_args;
+int ds5_hip_paged_attention(ds5_hip_ctx* ctx, const ds5_paged_attention_args* args);
+
 /* ========================================================================
- * 5. Bench/test utility (no reference counterpart)
+ * 5. Scores of tokens (no reference counterpart: the reference copies every
+ *    logit to the host, forward.zig:490-500)
+ * ======================================================================== */
+
+/* Per row of logits, the softmax's log probabilities without writing them all:
+ * logprobs = that of the row's target, entropy = -sum p log p (nats), and the
+ * top_n tokens by logit, descending (equal logits: the lower id first), with
+ * their log probabilities. Row r begins at element r * row_stride of logits and
+ * has vocab elements. Every output is optional (len 0; top_ids and top_logprobs
+ * go with top_n and must both be given when top_n > 0); targets is required with
+ * logprobs. A logit of -inf is a token of probability 0 (log probability -inf). A
+ * target outside [0, vocab) gives NaN. A row that holds a NaN, a +inf or no finite
+ * logit has no distribution: its outputs are NaN, its top ids -1. Sums are held
+ * in f32 relative to the row's maximum, which itself stays out of them, so that
+ * the log probability and the entropy of a row that is almost certain keep their
+ * relative accuracy. vocab is at most DS5_LOGPROBS_MAX_VOCAB, top_n at most
+ * DS5_LOGPROBS_MAX_TOP and at most vocab; views 4-byte aligned, no output
+ * overlapping logits. Uses the context workspace: run a shape once before
+ * capturing it in a graph. */
+#define DS5_LOGPROBS_MAX_VOCAB (1u << 21)
+#define DS5_LOGPROBS_MAX_TOP 32u
+typedef struct ds5_token_logprobs_args {
+    ds5_buf logits;       /* f32, rows of vocab elements every row_stride */
+    ds5_buf targets;      /* i32 [n_rows] (with logprobs) */
+    ds5_buf logprobs;     /* optional f32 [n_rows] */
+    ds5_buf entropy;      /* optional f32 [n_rows] */
+    ds5_buf top_ids;      /* i32 [n_rows, top_n] */
+    ds5_buf top_logprobs; /* f32 [n_rows, top_n] */
+    uint32_t n_rows;
+    uint32_t vocab;
+    uint32_t row_stride;  /* elements, at least vocab */
+    uint32_t top_n;       /* 0: no alternatives */
+} ds5_token_logprobs_args;
+int ds5_hip_token_logprobs(ds5_hip_ctx* ctx, const ds5_token_logprobs_args* args);
+
+/* ========================================================================
+ * 6. Bench/test utility (no reference counterpart)
  * ======================================================================== */
 
 /* inv_freq[i] = theta^(-(2i)/head_dim), i < head_dim/2, exactly as the rope

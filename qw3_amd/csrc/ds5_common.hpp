@@ -426,6 +426,57 @@ int launch_prefill(ds5_hip_ctx* ctx, const PrefillLaunch& a);
 uint32_t prefill_splits(uint32_t cu_count, uint32_t pos, uint32_t n_tokens, uint32_t n_q_heads, uint32_t n_kv_heads,
                         uint32_t head_dim);
 
+// A ragged batch over the paged pool (k_paged.hip): sequence b holds the rows starts[b] ..
+// starts[b + 1] - 1, its newest tokens.
+struct PagedBatch {
+    const int32_t* page_table;  // [n_seqs, max_pages]
+    const int32_t* starts;      // [n_seqs + 1]
+    const int32_t* seq_lens;    // [n_seqs], the batch's rows included
+    uint32_t n_tokens, n_seqs, n_q_heads, n_kv_heads, head_dim;
+    uint32_t page_size, n_pages, max_pages, max_seq_len;
+};
+// inv[i] = theta^(-2i/head_dim) * freq_scale / (2 pi): turns per position of rope pair i
+struct RopeTurns {
+    double inv[64];
+};
+struct PagedAppendLaunch {
+    PagedBatch batch;
+    const float* q;  // null: none
+    const float* k;
+    const float* v;
+    const float* q_norm;  // null: no norm
+    const float* k_norm;
+    void* q_out;
+    bool q_f16;
+    f16* k_pool;
+    f16* v_pool;
+    float eps;
+    const RopeTurns* turns;
+};
+int launch_paged_append(ds5_hip_ctx* ctx, const PagedAppendLaunch& a);
+struct PagedAttentionLaunch {
+    PagedBatch batch;
+    const void* q;
+    bool q_f16;
+    const f16* k_pool;
+    const f16* v_pool;
+    float* out;
+    float scale;
+};
+int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a);
+
+// Log probabilities, entropy and top alternatives of rows of logits (k_logprobs.hip).
+struct LogprobsLaunch {
+    const float* logits;
+    const int32_t* targets;
+    float* logprobs;  // outputs null where not asked for
+    float* entropy;
+    int32_t* top_ids;
+    float* top_logprobs;
+    uint32_t n_rows, vocab, row_stride, top_n;
+};
+int launch_token_logprobs(ds5_hip_ctx* ctx, const LogprobsLaunch& a);
+
 int launch_fill_normal_f16(ds5_hip_ctx* ctx, f16* out, uint64_t n, uint64_t seed);
 int launch_stream_read(ds5_hip_ctx* ctx, const void* src, uint64_t len, uint32_t* sink);
 int launch_empty(ds5_hip_ctx* ctx, uint32_t n_workgroups);

@@ -142,6 +142,36 @@ const RopeTable* rope_table_for(float theta, uint32_t head_dim) {
     return &cache.table;
 }
 
+struct TurnsCache {
+    float theta = NAN, freq_scale = NAN;
+    uint32_t head_dim = 0;
+    RopeTurns turns;
+};
+
+const RopeTurns* rope_turns_for(float theta, float freq_scale, uint32_t head_dim) {
+    static thread_local TurnsCache cache;
+    if (!(cache.theta == theta) || !(cache.freq_scale == freq_scale) || cache.head_dim != head_dim) {
+        for (uint32_t i = 0; i < 64; i++)
+            cache.turns.inv[i] = i < head_dim / 2 ? pow((double)theta, -2.0 * i / head_dim) * (double)freq_scale /
+                                                        6.283185307179586476925286766559
+                                                  : 0.0;
+        cache.theta = theta;
+        cache.freq_scale = freq_scale;
+        cache.head_dim = head_dim;
+    }
+    return &cache.turns;
+}
+
+// The product of sizes, or the largest value where it does not fit 64 bits (which no view covers).
+uint64_t size_of(std::initializer_list<uint64_t> factors) {
+    uint64_t n = 1;
+    for (uint64_t f : factors)
+        if (__builtin_mul_overflow(n, f, &n)) return UINT64_MAX;
+    return n;
+}
+
+bool aligned4(ds5_buf b) { return ((uintptr_t)ds5_ptr(b) & 3u) == 0; }
+
 // Runs after the preconditions, so shape errors are reported even without a
 // device context (a null context then fails with DeviceFailure).
 int set_device(ds5_hip_ctx* ctx) {
@@ -1026,6 +1056,184 @@ int ds5_hip_paged_decode(ds5_hip_ctx* ctx, const ds5_paged_decode_args* a) {
     l.fused = true;
     l.table = rope_table_for(a->theta, a->head_dim);
     return launch_decode(ctx, l);
+}
+
+// Preconditions of a ragged batch over the paged pool, and the batch.
+static int check_paged_batch(ds5_hip_ctx* ctx, const char* op, const PagedBatch& p, ds5_buf k_pool, ds5_buf v_pool,
+                             ds5_buf page_table, ds5_buf starts, ds5_buf seq_lens, uint32_t q_dtype) {
+    if (q_dtype != DS5_DTYPE_F32 && q_dtype != DS5_DTYPE_F16)
+        return ds5_fail(ctx, DS5_UNSUPPORTED_DTYPE, "%s: q_dtype %u (f32 and f16 are supported)", op, q_dtype);
+    if (p.n_kv_heads == 0) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: n_kv_heads == 0", op);
+    if (p.head_dim != 64 && p.head_dim != 128)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: head_dim must be 64 or 128", op);
+    if (p.page_size == 0 || p.n_pages == 0 || p.max_pages == 0)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: empty page geometry", op);
+    if (p.page_size % 16 != 0)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: page_size must be a multiple of 16", op);
+    if (p.max_seq_len > (uint64_t)p.max_pages * p.page_size)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: max_seq_len exceeds max_pages * page_size", op);
+    if (p.max_seq_len > INT32_MAX || p.n_tokens > INT32_MAX)  // what the i32 lengths and starts can say
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: max_seq_len or n_tokens above 2^31 - 1", op);
+    const uint64_t pool = size_of({p.n_kv_heads, p.n_pages, p.page_size, p.head_dim, 2});
+    if (!covers(k_pool, pool) || !covers(v_pool, pool))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: pool too small", op);
+    if (!covers(page_table, size_of({p.n_seqs, p.max_pages, 4})) || !covers(starts, ((uint64_t)p.n_seqs + 1) * 4) ||
+        !covers(seq_lens, (uint64_t)p.n_seqs * 4))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: page_table/starts/seq_lens too small", op);
+    if (!aligned16(k_pool) || !aligned16(v_pool) || !aligned4(page_table) || !aligned4(starts) || !aligned4(seq_lens))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: unaligned view", op);
+    return DS5_OK;
+}
+
+int ds5_hip_paged_append(ds5_hip_ctx* ctx, const ds5_paged_append_args* a) {
+    if (!a) return DS5_SHAPE_MISMATCH;
+    const char* op = "paged_append";
+    PagedAppendLaunch l{};
+    l.batch = PagedBatch{(const int32_t*)ds5_ptr(a->page_table), (const int32_t*)ds5_ptr(a->starts),
+                         (const int32_t*)ds5_ptr(a->seq_lens), a->n_tokens, a->n_seqs, a->n_q_heads, a->n_kv_heads,
+                         a->head_dim, a->page_size, a->n_pages, a->max_pages, a->max_seq_len};
+    if (int rc = check_paged_batch(ctx, op, l.batch, a->k_pool, a->v_pool, a->page_table, a->starts, a->seq_lens, a->q_dtype))
+        return rc;
+    const bool with_q = a->q.len != 0;
+    const uint64_t T = a->n_tokens, hd = a->head_dim;
+    const uint64_t q_bytes = size_of({T, a->n_q_heads, hd, 4}), kv_bytes = size_of({T, a->n_kv_heads, hd, 4});
+    const uint64_t out_bytes = a->q_dtype == DS5_DTYPE_F16 ? q_bytes / 2 : q_bytes;
+    const uint64_t pool_bytes = size_of({a->n_kv_heads, a->n_pages, a->page_size, hd, 2});
+    if (with_q && a->n_q_heads == 0) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: n_q_heads == 0", op);
+    if (with_q && (!covers(a->q, q_bytes) || !covers(a->q_out, out_bytes)))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: q/q_out too small", op);
+    if (!covers(a->k, kv_bytes) || !covers(a->v, kv_bytes)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: k/v too small", op);
+    if ((a->q_norm.len && !covers(a->q_norm, hd * 4)) || (a->k_norm.len && !covers(a->k_norm, hd * 4)))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: norm weights too small", op);
+    if (!aligned16(a->k) || !aligned16(a->v) || (a->q_norm.len && !aligned16(a->q_norm)) ||
+        (a->k_norm.len && !aligned16(a->k_norm)) || (with_q && (!aligned16(a->q) || !aligned16(a->q_out))))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: views must be 16-byte aligned", op);
+    if (T == 0 || a->n_seqs == 0) return DS5_OK;
+    // what is written must not be read as something else by another workgroup
+    struct View {
+        ds5_buf b;
+        uint64_t n;
+    };
+    const View in[] = {{a->k, kv_bytes}, {a->v, kv_bytes}, {a->q, with_q ? q_bytes : 0},
+                       {a->q_norm, a->q_norm.len ? hd * 4 : 0}, {a->k_norm, a->k_norm.len ? hd * 4 : 0},
+                       {a->page_table, (uint64_t)a->n_seqs * a->max_pages * 4}, {a->starts, ((uint64_t)a->n_seqs + 1) * 4},
+                       {a->seq_lens, (uint64_t)a->n_seqs * 4}};
+    const View out[] = {{a->k_pool, pool_bytes}, {a->v_pool, pool_bytes}, {a->q_out, with_q ? out_bytes : 0}};
+    const bool in_place = with_q && a->q_dtype == DS5_DTYPE_F32 && ds5_ptr(a->q) == ds5_ptr(a->q_out);
+    for (int o = 0; o < 3; o++) {
+        if (out[o].n == 0) continue;
+        for (int i = 0; i < 8; i++)
+            if (in[i].n && !(o == 2 && i == 2 && in_place) && !disjoint(out[o].b, out[o].n, in[i].b, in[i].n))
+                return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: an output overlaps an input", op);
+        for (int i = 0; i < o; i++)
+            if (!disjoint(out[o].b, out[o].n, out[i].b, out[i].n))
+                return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: outputs overlap", op);
+    }
+    if (int rc = set_device(ctx)) return rc;
+    l.q = with_q ? (const float*)ds5_ptr(a->q) : nullptr;
+    l.k = (const float*)ds5_ptr(a->k);
+    l.v = (const float*)ds5_ptr(a->v);
+    l.q_norm = a->q_norm.len ? (const float*)ds5_ptr(a->q_norm) : nullptr;
+    l.k_norm = a->k_norm.len ? (const float*)ds5_ptr(a->k_norm) : nullptr;
+    l.q_out = ds5_ptr(a->q_out);
+    l.q_f16 = a->q_dtype == DS5_DTYPE_F16;
+    l.k_pool = (f16*)ds5_ptr(a->k_pool);
+    l.v_pool = (f16*)ds5_ptr(a->v_pool);
+    l.eps = a->eps;
+    l.turns = rope_turns_for(a->theta, a->freq_scale, a->head_dim);
+    return launch_paged_append(ctx, l);
+}
+
+int ds5_hip_paged_attention(ds5_hip_ctx* ctx, const ds5_paged_attention_args* a) {
+    if (!a) return DS5_SHAPE_MISMATCH;
+    const char* op = "paged_attention";
+    PagedAttentionLaunch l{};
+    l.batch = PagedBatch{(const int32_t*)ds5_ptr(a->page_table), (const int32_t*)ds5_ptr(a->starts),
+                         (const int32_t*)ds5_ptr(a->seq_lens), a->n_tokens, a->n_seqs, a->n_q_heads, a->n_kv_heads,
+                         a->head_dim, a->page_size, a->n_pages, a->max_pages, a->max_seq_len};
+    if (int rc = check_paged_batch(ctx, op, l.batch, a->k_pool, a->v_pool, a->page_table, a->starts, a->seq_lens, a->q_dtype))
+        return rc;
+    if (a->n_q_heads == 0 || a->n_q_heads % a->n_kv_heads != 0)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: n_q_heads is not a positive multiple of n_kv_heads", op);
+    if (a->n_seqs > DS5_PAGED_MAX_SEQS)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: more than %u sequences", op, DS5_PAGED_MAX_SEQS);
+    const uint64_t T = a->n_tokens, out_bytes = size_of({T, a->n_q_heads, a->head_dim, 4});
+    const uint64_t q_bytes = a->q_dtype == DS5_DTYPE_F16 ? out_bytes / 2 : out_bytes;
+    if (!covers(a->q, q_bytes) || !covers(a->out, out_bytes))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: q/out too small", op);
+    if (!aligned16(a->q) || !aligned16(a->out))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: views must be 16-byte aligned", op);
+    if (T * (a->n_q_heads / a->n_kv_heads) > INT32_MAX)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: too many query rows", op);
+    if (T == 0 || a->n_seqs == 0) return DS5_OK;
+    const uint64_t pool_bytes = size_of({a->n_kv_heads, a->n_pages, a->page_size, a->head_dim, 2});
+    if (!disjoint(a->out, out_bytes, a->q, q_bytes) || !disjoint(a->out, out_bytes, a->k_pool, pool_bytes) ||
+        !disjoint(a->out, out_bytes, a->v_pool, pool_bytes) ||
+        !disjoint(a->out, out_bytes, a->page_table, (uint64_t)a->n_seqs * a->max_pages * 4) ||
+        !disjoint(a->out, out_bytes, a->starts, ((uint64_t)a->n_seqs + 1) * 4) ||
+        !disjoint(a->out, out_bytes, a->seq_lens, (uint64_t)a->n_seqs * 4))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: out overlaps an input", op);
+    if (int rc = set_device(ctx)) return rc;
+    l.q = ds5_ptr(a->q);
+    l.q_f16 = a->q_dtype == DS5_DTYPE_F16;
+    l.k_pool = (const f16*)ds5_ptr(a->k_pool);
+    l.v_pool = (const f16*)ds5_ptr(a->v_pool);
+    l.out = (float*)ds5_ptr(a->out);
+    l.scale = a->scale;
+    return launch_paged_attention(ctx, l);
+}
+
+int ds5_hip_token_logprobs(ds5_hip_ctx* ctx, const ds5_token_logprobs_args* a) {
+    if (!a) return DS5_SHAPE_MISMATCH;
+    const char* op = "token_logprobs";
+    const uint64_t n = a->n_rows, V = a->vocab, top = a->top_n;
+    if (V == 0 || V > DS5_LOGPROBS_MAX_VOCAB)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: vocab %u (1..%u)", op, a->vocab, DS5_LOGPROBS_MAX_VOCAB);
+    if (a->row_stride < V) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: row_stride below vocab", op);
+    if (top > DS5_LOGPROBS_MAX_TOP || top > V)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: top_n %u (at most %u and vocab)", op, a->top_n, DS5_LOGPROBS_MAX_TOP);
+    if (n > INT32_MAX || n * a->row_stride > (1ull << 61)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: too many rows", op);
+    const uint64_t logit_bytes = n ? ((n - 1) * a->row_stride + V) * 4 : 0;
+    if (!covers(a->logits, logit_bytes)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: logits too small", op);
+    if (a->logprobs.len && !covers(a->targets, n * 4)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: targets too small", op);
+    const struct {
+        ds5_buf b;
+        uint64_t n;
+        const char* name;
+    } out[] = {{a->logprobs, a->logprobs.len ? n * 4 : 0, "logprobs"}, {a->entropy, a->entropy.len ? n * 4 : 0, "entropy"},
+               {a->top_ids, n * top * 4, "top_ids"}, {a->top_logprobs, n * top * 4, "top_logprobs"}};
+    for (const auto& o : out) {
+        if (!covers(o.b, o.n)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: %s too small", op, o.name);
+        if (o.n && !aligned4(o.b)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: %s is not 4-byte aligned", op, o.name);
+    }
+    if (!aligned4(a->logits) || (a->logprobs.len && !aligned4(a->targets)))
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: logits and targets must be 4-byte aligned", op);
+    if (n == 0) return DS5_OK;
+    bool any = false;
+    for (int i = 0; i < 4; i++) {
+        if (!out[i].n) continue;
+        any = true;
+        if (!disjoint(out[i].b, out[i].n, a->logits, logit_bytes) ||
+            (a->logprobs.len && !disjoint(out[i].b, out[i].n, a->targets, n * 4)))
+            return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: %s overlaps an input", op, out[i].name);
+        for (int j = 0; j < i; j++)
+            if (out[j].n && !disjoint(out[i].b, out[i].n, out[j].b, out[j].n))
+                return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: outputs overlap", op);
+    }
+    if (!any) return DS5_OK;
+    if (int rc = set_device(ctx)) return rc;
+    LogprobsLaunch l{};
+    l.logits = (const float*)ds5_ptr(a->logits);
+    l.targets = (const int32_t*)ds5_ptr(a->targets);
+    l.logprobs = a->logprobs.len ? (float*)ds5_ptr(a->logprobs) : nullptr;
+    l.entropy = a->entropy.len ? (float*)ds5_ptr(a->entropy) : nullptr;
+    l.top_ids = (int32_t*)ds5_ptr(a->top_ids);
+    l.top_logprobs = (float*)ds5_ptr(a->top_logprobs);
+    l.n_rows = a->n_rows;
+    l.vocab = a->vocab;
+    l.row_stride = a->row_stride;
+    l.top_n = a->top_n;
+    return launch_token_logprobs(ctx, l);
 }
 
 int ds5_hip_rope_table(float theta, uint32_t head_dim, float* out) {

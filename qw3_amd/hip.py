@@ -177,6 +177,32 @@ class PagedDecodeArgs(C.Structure):
                [(n, C.c_float) for n in ("eps", "theta", "freq_scale", "scale")]
 
 
+_PAGED_BATCH = [(n, C.c_uint32) for n in ("q_dtype", "n_tokens", "n_seqs", "n_q_heads", "n_kv_heads", "head_dim", "page_size",
+                                          "n_pages", "max_pages", "max_seq_len")]
+
+
+class PagedAppendArgs(C.Structure):
+    """ds5_paged_append_args; q, q_norm and k_norm are optional (Buf())."""
+    _fields_ = [(n, Buf) for n in ("q", "k", "v", "q_norm", "k_norm", "q_out", "k_pool", "v_pool", "page_table", "starts",
+                                   "seq_lens")] + _PAGED_BATCH + \
+               [(n, C.c_float) for n in ("eps", "theta", "freq_scale")]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [(n, Buf) for n in ("q", "k_pool", "v_pool", "page_table", "starts", "seq_lens", "out")] + _PAGED_BATCH + \
+               [("scale", C.c_float)]
+
+
+PAGED_MAX_SEQS = 1024  # DS5_PAGED_MAX_SEQS
+LOGPROBS_MAX_VOCAB = 1 << 21  # DS5_LOGPROBS_MAX_VOCAB
+LOGPROBS_MAX_TOP = 32  # DS5_LOGPROBS_MAX_TOP
+
+
+class TokenLogprobsArgs(C.Structure):
+    _fields_ = [(n, Buf) for n in ("logits", "targets", "logprobs", "entropy", "top_ids", "top_logprobs")] + \
+               [(n, C.c_uint32) for n in ("n_rows", "vocab", "row_stride", "top_n")]
+
+
 # Every symbol include/ds5_hip.h declares, with its ctypes signature.
 _P = C.c_void_p
 SIGNATURES = {
@@ -215,6 +241,9 @@ SIGNATURES = {
     "ds5_hip_attention_step_noalloc": ([_P, C.POINTER(AttentionStepArgs)], C.c_int),
     "ds5_hip_attention_block": ([_P, C.POINTER(AttentionBlockArgs)], C.c_int),
     "ds5_hip_paged_decode": ([_P, C.POINTER(PagedDecodeArgs)], C.c_int),
+    "ds5_hip_paged_append": ([_P, C.POINTER(PagedAppendArgs)], C.c_int),
+    "ds5_hip_paged_attention": ([_P, C.POINTER(PagedAttentionArgs)], C.c_int),
+    "ds5_hip_token_logprobs": ([_P, C.POINTER(TokenLogprobsArgs)], C.c_int),
     "ds5_hip_rope_table": ([C.c_float, C.c_uint32, C.c_void_p], C.c_int),
     "ds5_hip_fill_normal_f16": ([_P, Buf, C.c_uint64, C.c_uint64], C.c_int),
     "ds5_hip_copy_device": ([_P, Buf, Buf, C.c_uint64], C.c_int),
@@ -497,3 +526,20 @@ def rope_table(theta: float, head_dim: int) -> np.ndarray:
 def pagedDecode(ctx: Ctx, args: PagedDecodeArgs) -> None:
     """Batched decode over a paged f16 pool (one new token per sequence)."""
     ctx.check(LIB.ds5_hip_paged_decode(ctx.handle, C.byref(args)))
+
+
+def pagedAppend(ctx: Ctx, args: PagedAppendArgs) -> None:
+    """Norm, rotation and append of a ragged batch's k and v into the paged pool, and its q for
+    pagedAttention. No reference counterpart."""
+    ctx.check(LIB.ds5_hip_paged_append(ctx.handle, C.byref(args)))
+
+
+def pagedAttention(ctx: Ctx, args: PagedAttentionArgs) -> None:
+    """Causal attention of a ragged batch (one or many new tokens per sequence) over the paged
+    pool. No reference counterpart."""
+    ctx.check(LIB.ds5_hip_paged_attention(ctx.handle, C.byref(args)))
+
+
+def tokenLogprobs(ctx: Ctx, args: TokenLogprobsArgs) -> None:
+    """Log probabilities of target tokens, entropy and the top alternatives of rows of logits."""
+    ctx.check(LIB.ds5_hip_token_logprobs(ctx.handle, C.byref(args)))
