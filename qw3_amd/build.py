@@ -30,12 +30,13 @@ CXXFLAGS = [
 ]
 
 
-# Per-file extra flags. k_prefill.hip: MFMA accumulators in VGPRs. The attention
+# Per-file extra flags. k_prefill.hip, k_paged.hip: MFMA accumulators in VGPRs. The attention
 # kernel reads its scores with VALU instructions, which cannot take AGPRs; with
 # the AGPR form the backend copied the O accumulators between the register files
 # every round.
 EXTRA_FLAGS = {
     "k_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "k_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -65,8 +65,8 @@ struct ds5_hip_ctx {
     void* scratch = nullptr;
     size_t scratch_bytes = 0;
     bool use_scratch = false;
-    // kSplitBytesMax bytes for the partial results of an attention launch split over its keys
-    // (prefill, f32 caches), allocated at init: whether a call splits then depends on its shape
+    // kSplitBytesMax + kSplitStateBytes for the partial results of an attention launch split over
+    // its keys (prefill, f32 caches, paged batches), allocated at init: whether a call splits then depends on its shape
     // alone, captured or not, whatever ran before it. Null if there was no memory for it: such
     // a context runs those launches unsplit.
     void* split_buf = nullptr;
@@ -103,6 +103,8 @@ int ds5_hip_status(ds5_hip_ctx* ctx, hipError_t err, const char* what);
 int ds5_after_launch(ds5_hip_ctx* ctx, const char* what);
 int ds5_workspace(ds5_hip_ctx* ctx, size_t bytes, void** out);
 constexpr size_t kSplitBytesMax = 32u << 20;
+// Behind them in split_buf: references, sums and tile descriptors of a paged attention's parts.
+constexpr size_t kSplitStateBytes = 1u << 20;
 // The most splits of `rows` rows of partials that kSplitBytesMax holds.
 inline uint32_t ds5_max_splits(uint64_t rows, uint32_t head_dim) {
     const uint64_t row = rows * (head_dim + 2) * sizeof(float);

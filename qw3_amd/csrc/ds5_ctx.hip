@@ -130,7 +130,7 @@ int ds5_hip_init(int device_index, ds5_hip_ctx** out) {
     if (!rc) rc = ds5_hip_status(ctx, hipEventCreate(&ctx->ev_begin), "hipEventCreate");
     if (!rc) rc = ds5_hip_status(ctx, hipEventCreate(&ctx->ev_end), "hipEventCreate");
     if (!rc) rc = ds5_scratch_init(ctx);
-    if (!rc && hipMalloc(&ctx->split_buf, kSplitBytesMax) != hipSuccess) {
+    if (!rc && hipMalloc(&ctx->split_buf, kSplitBytesMax + kSplitStateBytes) != hipSuccess) {
         (void)hipGetLastError();
         ctx->split_buf = nullptr;
     }

@@ -5,6 +5,7 @@
 
 #include "ds5_common.hpp"
 #include "ds5_index.h"
+#include "ds5_paged_index.h"
 
 extern "C" {
 
@@ -154,5 +155,59 @@ uint32_t ds5_index_af_store(uint32_t lim, uint32_t start, uint32_t chunk) {
     return (uint32_t)ds5idx::af_store(lim, start, chunk);
 }
 uint32_t ds5_index_af_row_splits(uint32_t lim, uint32_t chunk) { return ds5idx::af_row_splits(lim, chunk); }
+
+
+// The ragged batch's parts, workgroup by workgroup, as paged_attention_kernel walks them.
+uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* before, uint32_t group, uint32_t n_kv_heads,
+                            uint32_t grid, int whole, uint32_t max, uint32_t* out) {
+    using namespace ds5idx;
+    auto seq = [&](uint32_t b) { return PbSeq{n[b], before[b]}; };
+    uint64_t per_head = 0;
+    for (uint32_t b = 0; b < n_seqs; b++) per_head += n[b] ? pb_seq_work(seq(b), group) : 0;
+    const uint64_t total = per_head * n_kv_heads;
+    if (!total) return 0;
+    const uint32_t n_wg = whole ? grid : pb_workgroups(total, group, grid);
+    const uint64_t snap = pb_snap(total, n_wg, group);
+    uint64_t line = 0;
+    auto cut = [&](uint32_t w) {
+        if (w == n_wg) return PbCut{n_kv_heads, 0, 0, 0};
+        const uint64_t x = pb_cut_at(total, w, n_wg), y = x % per_head;
+        PbCut c{(uint32_t)(x / per_head), 0, 0, 0};
+        uint64_t from = 0;
+        for (;; c.b++) {
+            const uint64_t work = n[c.b] ? pb_seq_work(seq(c.b), group) : 0;
+            if (y - from < work) break;
+            from += work;
+        }
+        pb_locate(seq(c.b), group, y - from, snap, whole != 0, c.j, c.k);
+        line = c.kvh * per_head + from + pb_before(seq(c.b), group, c.j);
+        return c;
+    };
+    uint32_t count = 0;
+    for (uint32_t w = 0; w < n_wg; w++) {
+        const PbCut stop = cut(w + 1);
+        PbCut at = cut(w);
+        bool at_end = false;
+        for (; !at_end && pb_next(at, stop, n_seqs, n_kv_heads, group, seq, at_end); at.j++, at.k = 0) {
+            const uint32_t ti = pb_tile_at(at.j, pb_tiles(seq(at.b), group));
+            const PbTile t = pb_tile(seq(at.b), group, ti);
+            const uint32_t end = at_end ? stop.k : t.kv;
+            const uint64_t tile_end = line + pb_tile_work(seq(at.b), group, ti);
+            if (count < max) {
+                const bool begins = at.k == 0 && end < t.kv;
+                const uint32_t row[10] = {w, at.kvh, at.b, ti, at.k, end, t.kv, t.row0, t.rows,
+                                          begins ? pb_last_cut(total, n_wg, tile_end - snap) : w};
+                for (int i = 0; i < 10; i++) out[10 * count + i] = row[i];
+            }
+            count++;
+            line = tile_end;
+        }
+    }
+    return count;
+}
+void ds5_index_pb_loads(uint32_t head_dim, int v, uint32_t* off) {
+    for (uint32_t b = 0; b < 16 * 2 * head_dim / 1024; b++)
+        for (int lane = 0; lane < 64; lane++) off[b * 64 + lane] = ds5idx::pb_load_off((int)head_dim, v != 0, (int)b, lane);
+}
 
 }  // extern "C"

@@ -11,7 +11,9 @@
 //   prefill_attention_kernel (k_prefill.hip): the lane offsets of a K/V tile's
 //     direct-to-LDS loads and their clamp, and the staged q and output rows;
 //   attn_f32_kernel (k_attn_f32.hip): a wavefront's query rows, the clamped positions of
-//     its loads, and which split writes a row where.
+//     its loads, and which split writes a row where;
+//   paged_attention_kernel (k_paged.hip): the tiles of a ragged batch, how the batch's work is
+//     cut over the workgroups, and the lane offsets of a row group's direct-to-LDS loads.
 #pragma once
 
 #include <stdint.h>
@@ -194,5 +196,111 @@ DS5_HD int af_store(uint32_t lim, uint32_t start, uint32_t chunk) {
 }
 // The splits that hold a partial result of the row (1: its only split wrote the output).
 DS5_HD uint32_t af_row_splits(uint32_t lim, uint32_t chunk) { return lim / chunk + 1; }
+
+// ---------------------------------------------------------------------------
+// paged_attention_kernel. A sequence's query rows of one kv head are its new tokens' q heads
+// of that group, row = token * group + head, in tiles of kPbRows; tile i attends the positions
+// below its last token's. The batch's work is one line: for each kv head, each sequence, each
+// tile in the order last, first, last but one, second, ... (a pair of them costs the same for
+// every pair), its positions. Workgroup w of n takes the part from w / n to (w + 1) / n of it.
+// Work is counted in positions * group, a tile's being its positions (taken as if every tile
+// were full) and kPbTileCost more. A cut inside a tile falls on a multiple of kPbUnit
+// positions of it, or on the tile's start or end where that is no further than `snap`.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 64;
+
+struct PbSeq {
+    uint32_t n, before;  // new tokens, and the tokens before them
+};
+struct PbTile {
+    uint32_t row0, rows, kv;  // first query row, rows, positions that the last of them attends
+};
+struct PbCut {
+    uint32_t kvh, b, j, k;  // kv head, sequence, the j-th tile of its order, position
+};
+
+DS5_HD uint32_t pb_tiles(PbSeq s, uint32_t group) { return (s.n * group + kPbRows - 1) / kPbRows; }
+DS5_HD uint64_t pb_tile_work(PbSeq s, uint32_t group, uint32_t tile) {
+    return (uint64_t)group * ((uint64_t)s.before + kPbTileCost) + (uint64_t)kPbRows * (tile + 1);
+}
+DS5_HD uint64_t pb_seq_work(PbSeq s, uint32_t group) {
+    const uint64_t nt = pb_tiles(s, group);
+    return nt * group * ((uint64_t)s.before + kPbTileCost) + kPbRows / 2 * nt * (nt + 1);
+}
+DS5_HD uint32_t pb_tile_at(uint32_t j, uint32_t nt) { return j % 2 ? j / 2 : nt - 1 - j / 2; }
+DS5_HD PbTile pb_tile(PbSeq s, uint32_t group, uint32_t tile) {
+    const uint32_t all = s.n * group, row0 = tile * kPbRows, end = umin(all, row0 + kPbRows);
+    return PbTile{row0, end - row0, s.before + (end - 1) / group + 1};
+}
+// The work before the j-th tile of a sequence's order.
+DS5_HD uint64_t pb_before(PbSeq s, uint32_t group, uint32_t j) {
+    const uint32_t nt = pb_tiles(s, group);
+    const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
+    return j / 2 * pair + (j % 2 ? pb_tile_work(s, group, nt - 1 - j / 2) : 0);
+}
+// The cut at y of a sequence's work: tile j of its order (j may be one past the last), position k.
+DS5_HD void pb_locate(PbSeq s, uint32_t group, uint64_t y, uint64_t snap, bool whole, uint32_t& j, uint32_t& k) {
+    const uint32_t nt = pb_tiles(s, group);
+    const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
+    j = (uint32_t)(y / pair) * 2;
+    uint64_t off = y % pair;
+    const uint64_t heavy = pb_tile_work(s, group, pb_tile_at(j, nt));
+    if (j + 1 < nt && off >= heavy) {
+        j++;
+        off -= heavy;
+    }
+    k = 0;
+    const uint32_t tile = pb_tile_at(j, nt);
+    const uint64_t w = pb_tile_work(s, group, tile);
+    if (whole) {  // cuts between tiles only
+        j += off * 2 >= w;
+        return;
+    }
+    if (off < snap) return;
+    if (w - off < snap) {
+        j++;
+        return;
+    }
+    const uint32_t kv = pb_tile(s, group, tile).kv;
+    k = umin((uint32_t)((double)kv * (double)off / (double)w), kv - 1) / kPbUnit * kPbUnit;
+}
+// The cut before workgroup w of n: x of a line of `work` (below 2^54, n below 2^9).
+DS5_HD uint64_t pb_cut_at(uint64_t work, uint32_t w, uint32_t n) { return work * w / n; }
+// The last workgroup whose cut is at most x (x below work).
+DS5_HD uint32_t pb_last_cut(uint64_t work, uint32_t n, uint64_t x) { return (uint32_t)(((x + 1) * n - 1) / work); }
+DS5_HD uint64_t pb_snap(uint64_t work, uint32_t n, uint32_t group) {
+    const uint64_t part = work / n / 16, least = (uint64_t)group * (kPbUnit / 2);
+    return part > least ? part : least;
+}
+// The workgroups that share a line of work: 2 kPbUnit positions of a tile each at least.
+DS5_HD uint32_t pb_workgroups(uint64_t work, uint32_t group, uint32_t grid) {
+    const uint64_t n = work / ((uint64_t)group * (2 * kPbUnit + kPbTileCost));
+    return n >= grid ? grid : n < 1 ? 1 : (uint32_t)n;
+}
+// Moves c on to the next tile that has rows; false where that is past the part that ends at `end`.
+// at_end: the part ends inside this tile, at position end.k. seq(b) gives sequence b.
+template <class Seq>
+DS5_HD bool pb_next(PbCut& c, const PbCut& end, uint32_t n_seqs, uint32_t n_kv_heads, uint32_t group, Seq seq, bool& at_end) {
+    while (c.kvh < n_kv_heads && (c.b >= n_seqs || c.j >= pb_tiles(seq(c.b), group))) {
+        c.j = c.k = 0;
+        if (++c.b >= n_seqs) {
+            c.b = 0;
+            c.kvh++;
+        }
+    }
+    at_end = c.kvh == end.kvh && c.b == end.b && c.j == end.j;
+    if (c.kvh >= n_kv_heads || (at_end && end.k == 0)) return false;
+    return c.kvh < end.kvh || (c.kvh == end.kvh && (c.b < end.b || (c.b == end.b && c.j <= end.j)));
+}
+// Lane's byte offset, from the first row of a group of 16 rows of 2 D bytes, of its 16 bytes of
+// direct-to-LDS load b (LDS bytes 1024 b + 16 lane of the group): 16-byte chunk c of row r lies
+// in the row's slot c ^ (pb_swz of the row).
+DS5_HD uint32_t pb_swz(int D, bool v, uint32_t r) {
+    return v ? 4 * (D == 128 ? r & 3 : (r >> 1) & 1) : D == 128 ? r & 15 : (r >> 1) & 7;
+}
+DS5_HD uint32_t pb_load_off(int D, bool v, int b, int lane) {
+    const uint32_t at = 1024 * b + 16 * lane, r = at / (2 * D), slot = at % (2 * D) / 16;
+    return r * (2 * D) + (slot ^ pb_swz(D, v, r)) * 16;
+}
 
 }  // namespace ds5idx

@@ -145,50 +145,567 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppen
 }
 
 // ---------------------------------------------------------------------------
-// Attention: a wavefront per (row, q head), 64 positions at a time: each lane one position's
-// score, then the weights' sum over the positions with two or one elements of v per lane.
+// Attention
 // ---------------------------------------------------------------------------
+constexpr int kThreads = 512, kWaves = 8;
+constexpr int kRows = ds5idx::kPbRows, kNarrow = ds5idx::kPbNarrow;
+constexpr uint32_t kMaxSeqs = DS5_PAGED_MAX_SEQS;
+constexpr uint32_t kMaxGrid = 256;
+// Weights are exp2(score - reference): the reference starts 2^8 below the row's maximum and moves
+// when a weight would pass 2^15, so that in f16 hi + lo a weight keeps its 22 bits down to 2^-22
+// of the largest and counts down to 2^-33 of it.
+constexpr float kHead = 8.0f, kMove = 15.0f;
+
+struct MergeDesc {
+    uint32_t last;  // the tile's parts: this workgroup's head part, then workgroups w + 1 .. last
+    uint32_t rows;  // 0: nothing to merge
+    uint32_t row0, kvh, token0;
+};
+
+struct AttnParams {
+    PagedAttentionLaunch a;
+    uint32_t group;
+    bool whole;        // no tile is cut
+    float* part_o;     // [2 * workgroups, kRows, D]: slot 2 w the part that workgroup w continues, 2 w + 1 the one it begins
+    float2* part_ml;   // [2 * workgroups, kRows]: reference and sum
+    MergeDesc* descs;  // [workgroups]
+};
+
+__device__ __forceinline__ f16x4 lds_read_tr16(const char* lds_ptr) {
+    typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 v4h;
+    typedef __attribute__((address_space(3))) v4h lds_v4h;
+    const v4h r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h*)(lds_ptr));
+    return __builtin_bit_cast(f16x4, r);
+}
+
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // at most N vector-memory operations of the wavefront in flight
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Hi and lo f16 of two values: 22 bits of each.
+__device__ __forceinline__ void split2(float x0, float x1, f16x2& hi, f16x2& lo) {
+    hi = f16x2{(f16)x0, (f16)x1};
+    lo = f16x2{(f16)(x0 - (float)hi[0]), (f16)(x1 - (float)hi[1])};
+}
+
+// A scalar load of one i32 (the scalar cache holds nothing of before the launch).
+__device__ __forceinline__ int32_t scalar_i32(const int32_t* p, uint64_t i) {
+    return ((const __attribute__((address_space(4))) int32_t*)p)[i];
+}
+
 template <int D, bool Q16>
-__global__ __launch_bounds__(256) void paged_attention_kernel(PagedAttentionLaunch a) {
-    __shared__ float s_q[4][D];
-    const PagedBatch& p = a.batch;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t item = (uint64_t)blockIdx.x * 4 + wave;
-    const uint32_t t = (uint32_t)(item / p.n_q_heads), h = (uint32_t)(item % p.n_q_heads);
-    if (t >= p.n_tokens) return;
-    const uint32_t kvh = h / (p.n_q_heads / p.n_kv_heads);
-    const uint64_t slots = (uint64_t)p.n_pages * p.page_size;
-    const uint64_t row = ((uint64_t)t * p.n_q_heads + h) * D;
-    const RowInfo r = find_row(p, t, lane);
-    if (!r.held) return;
-    for (uint32_t i = lane; i < D; i += 64) s_q[wave][i] = Q16 ? (float)((const f16*)a.q)[row + i] : ((const float*)a.q)[row + i];
-    __builtin_amdgcn_wave_barrier();
-    const uint32_t L = r.ok ? r.pos + 1 : 0;
-    float mx = -INFINITY, l = 0.0f, o[D / 64] = {};
-    bool bad = !r.ok;
-    for (uint32_t j0 = 0; j0 < L; j0 += 64) {
-        const uint32_t j = min(j0 + lane, L - 1);
-        const int32_t pg = p.page_table[(uint64_t)r.b * p.max_pages + j / p.page_size];
-        const bool in = pg >= 0 && (uint32_t)pg < p.n_pages;
-        bad = bad || !in;
-        const uint64_t at = (uint64_t)kvh * slots + (uint64_t)(in ? pg : 0) * p.page_size + j % p.page_size;
-        float s = 0.0f;
-        for (int i = 0; i < D; i++) s += s_q[wave][i] * (float)a.k_pool[at * D + i];
-        s = j0 + lane < L ? s * a.scale : -INFINITY;
-        const float m_new = fmaxf(mx, wave_allreduce(s, OpMax{}));
-        const float alpha = expf(mx - m_new), w = expf(s - m_new);
-        l = l * alpha + wave_allreduce(w, OpAdd{});
-        for (int e = 0; e < D / 64; e++) o[e] *= alpha;
-        mx = m_new;
-        const uint32_t n = min(64u, L - j0);
-        for (uint32_t k = 0; k < n; k++) {
-            const float wk = __shfl(w, (int)k, 64);
-            const uint64_t ak = __shfl(at, (int)k, 64);
-            for (int e = 0; e < D / 64; e++) o[e] += wk * (float)a.v_pool[ak * D + lane + 64 * e];
+struct Attn {
+    static constexpr int KS = D / 16, DT = D / 32, RB = 2 * D;
+    static constexpr int NB = 16 * RB / 1024;      // direct-to-LDS loads of a group of 16 rows
+    static constexpr int HALF = 32 * RB;           // bytes of 32 rows
+    static constexpr int BUF = 2 * kRows * RB;     // wide: K then V of 128 positions
+    static constexpr int AREA = kWaves * 2 * HALF; // = 2 * BUF
+    static constexpr int CH = D / 4;               // float4 of an O row
+
+    f32x16 O[DT];
+    f16x8 qh[KS], ql[Q16 ? 1 : KS];
+    float fac;       // score = product * fac, log2 units
+    float m, l;      // reference, this lane's part of the sum
+    uint32_t lim;    // the row's last position
+    uint32_t koff[NB], voff[NB];
+
+    // Loads the 16 rows from `row` of the pool (rows of RB bytes) into 16 * RB bytes of LDS.
+    __device__ __forceinline__ static void load_group(uint32_t lds, const f16* row, const uint32_t* off) {
+        const uint64_t v = (uint64_t)row;
+        const uint64_t base = ((uint64_t)uniform((uint32_t)(v >> 32)) << 32) | uniform((uint32_t)v);
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[b]), "s"(base),
+                         "s"(uniform(lds + 1024 * b))
+                         : "m0", "memory");
+    }
+
+    // One block of 32 positions from key0, its K and V rows in LDS: scores, weights, sums.
+    template <bool MASK>
+    __device__ __forceinline__ void block(const char* sk, const char* sv, uint32_t key0, uint32_t end, int lane) {
+        const int r32 = lane & 31, h = lane >> 5, g16 = lane >> 4, i16 = lane & 15;
+        f32x16 S;
+        const char* krow = sk + r32 * RB;
+        const uint32_t kx = (ds5idx::pb_swz(D, false, r32) ^ h) * 16;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const f16x8 k = *(const f16x8*)(krow + (kx ^ (32 * ks)));
+            if (ks == 0) S = mfma_32x32x16(k, qh[0], f32x16{});
+            else S = mfma_32x32x16(k, qh[ks], S);
+            if constexpr (!Q16) S = mfma_32x32x16(k, ql[ks], S);
+        }
+        // lane (r32, h): score e is position key0 + 8 (e / 4) + 4 h + e % 4 of row r32
+        float t[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) t[e] = S[e] * fac;
+        if constexpr (MASK) {
+            const int seen = (int)min(lim, end - 1) - (int)key0 - 4 * h;
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (8 * (e / 4) + e % 4 > seen) t[e] = -INFINITY;
+        }
+        float mx = t[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) mx = fmaxf(mx, t[e]);
+        mx = swap32_op(mx, OpMax{});
+        if (__ballot(mx > m + kMove) != 0) {  // (m is -inf before the row's first score)
+            const float m_new = mx > m + kMove ? mx - kHead : m;
+            const float alpha = m_new == m ? 1.0f : fast_exp2(m - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) O[dt] *= alpha;
+            m = m_new;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;  // a row that has seen nothing: weights exp2(-inf)
+        float p[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) p[e] = fast_exp2(t[e] - ref);
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) sum += (p[e] + p[e + 1]) + (p[e + 2] + p[e + 3]);
+        l += sum;
+        f16x8 ph[2], pl[2];
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+            f16x2 hi, lo;
+            split2(p[e], p[e + 1], hi, lo);
+            ph[e / 8][e % 8] = hi[0], ph[e / 8][e % 8 + 1] = hi[1];
+            pl[e / 8][e % 8] = lo[0], pl[e / 8][e % 8 + 1] = lo[1];
+        }
+        // V^T operand of positions 16 s + [0, 16): the transpose read gives lane i of 16 column i
+        // of 4 rows; element jj of the operand is position 16 s + 8 (jj / 4) + 4 h + jj % 4
+        const char* vrow = sv + (4 * (g16 >> 1) + (i16 >> 2)) * RB;
+        const uint32_t vx = (2 * (g16 & 1) + ((i16 & 3) >> 1)) * 16 + 8 * (i16 & 1) + 16 * ds5idx::pb_swz(D, true, i16 >> 2);
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) {
+                const f16x4 a = lds_read_tr16(vrow + 16 * s * RB + (vx ^ (64 * dt)));
+                const f16x4 b = lds_read_tr16(vrow + (16 * s + 8) * RB + (vx ^ (64 * dt)));
+                const f16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                O[dt] = mfma_32x32x16(v, ph[s], O[dt]);
+                O[dt] = mfma_32x32x16(v, pl[s], O[dt]);
+            }
+    }
+
+    // V rows of a block from position `end` on to zero (their weights are 0, what they hold may be
+    // anything), and with CLEAN every infinity and NaN: true if there was one. The wavefronts that
+    // share the rows write the same values.
+    __device__ __forceinline__ static void zero_tail(char* sv, uint32_t key0, uint32_t end, int lane) {
+        for (int c = lane; c < 32 * RB / 16; c += 64)
+            if (key0 + c / (RB / 16) >= end) *(u32x4*)(sv + 16 * c) = u32x4{0u, 0u, 0u, 0u};
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ __forceinline__ static bool clean(char* sv, int lane) {
+        bool found = false;
+        for (int c = lane; c < 32 * RB / 16; c += 64) {
+            u32x4 v = *(const u32x4*)(sv + 16 * c);
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if ((v[i] & 0x7c00u) == 0x7c00u) v[i] &= 0xffff0000u, odd = true;
+                if ((v[i] & 0x7c000000u) == 0x7c000000u) v[i] &= 0xffffu, odd = true;
+            }
+            if (odd) *(u32x4*)(sv + 16 * c) = v;
+            found = found || odd;
+        }
+        __builtin_amdgcn_wave_barrier();
+        return __ballot(found) != 0;
+    }
+};
+
+template <int D, bool Q16>
+__global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p) {
+    using A = Attn<D, Q16>;
+    constexpr int KS = A::KS, DT = A::DT, RB = A::RB, NB = A::NB, HALF = A::HALF, BUF = A::BUF;
+    __shared__ __attribute__((aligned(1024))) char s_kv[A::AREA];
+    __shared__ uint32_t s_start[kMaxSeqs], s_n[kMaxSeqs], s_before[kMaxSeqs];
+    __shared__ float s_m[kWaves][32], s_l[kWaves][32];
+    __shared__ uint64_t s_scan[kWaves];
+    __shared__ uint32_t s_cut[2][3];
+    __shared__ uint64_t s_from;
+    __shared__ uint32_t s_bad, s_odd;
+
+    const PagedBatch& bt = p.a.batch;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, G = p.group;
+    const uint32_t wave = uniform(tid >> 6);
+    const uint32_t n_seqs = bt.n_seqs;
+    constexpr uint32_t kPoison = 0x80000000u;  // in s_before: the sequence's rows are NaN
+
+    // ---- the batch's sequences and their work
+    uint64_t work[kMaxSeqs / kThreads];
+    uint64_t mine = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSeqs / kThreads; i++) {
+        const uint32_t b = tid * (kMaxSeqs / kThreads) + i;
+        work[i] = 0;
+        if (b < n_seqs) {
+            const int64_t s0 = bt.starts[b], s1 = bt.starts[b + 1], len = bt.seq_lens[b];
+            const int64_t c0 = max(s0, (int64_t)0), c1 = min(s1, (int64_t)bt.n_tokens);
+            const uint32_t n = c1 > c0 ? (uint32_t)(c1 - c0) : 0;
+            const bool ok = c0 == s0 && c1 == s1 && len >= s1 - s0 && len <= (int64_t)bt.max_seq_len;
+            s_start[b] = (uint32_t)c0;
+            s_n[b] = n;
+            s_before[b] = ok ? (uint32_t)(len - n) : kPoison;
+            if (n) work[i] = ds5idx::pb_seq_work(ds5idx::PbSeq{n, ok ? (uint32_t)(len - n) : 0u}, G);
+        }
+        mine += work[i];
+    }
+    auto seq = [&](uint32_t b) { return ds5idx::PbSeq{s_n[b], s_before[b] & ~kPoison}; };
+    auto useq = [&](uint32_t b) { return ds5idx::PbSeq{uniform(s_n[b]), uniform(s_before[b]) & ~kPoison}; };
+    uint64_t upto = mine;  // inclusive over the wavefront
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t y = __shfl_up(upto, o, 64);
+        if ((int)lane >= o) upto += y;
+    }
+    if (lane == 63) s_scan[wave] = upto;
+    __syncthreads();
+    uint64_t base = 0, per_head = 0;
+    for (uint32_t w = 0; w < (uint32_t)kWaves; w++) {
+        base += w < wave ? s_scan[w] : 0;
+        per_head += s_scan[w];
+    }
+    const uint64_t total = per_head * bt.n_kv_heads;
+    const uint32_t grid = gridDim.x;
+    if (total == 0) {
+        if (tid == 0 && p.descs) p.descs[blockIdx.x].rows = 0;
+        return;
+    }
+    const uint32_t n_wg = p.whole ? grid : ds5idx::pb_workgroups(total, G, grid);
+    // A full grid's consecutive parts go to one XCD (workgroup i runs on XCD i % 8), so that a
+    // sequence's K and V come into few L2s.
+    const uint32_t wg = n_wg == grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
+    if (wg >= n_wg) {
+        if (tid == 0 && p.descs) p.descs[wg].rows = 0;
+        return;
+    }
+    const uint64_t snap = ds5idx::pb_snap(total, n_wg, G);
+    const uint64_t x0 = ds5idx::pb_cut_at(total, wg, n_wg), x1 = ds5idx::pb_cut_at(total, wg + 1, n_wg);
+    {
+        uint64_t from = base + upto - mine;
+#pragma unroll
+        for (uint32_t i = 0; i < kMaxSeqs / kThreads; i++) {
+            const uint32_t b = tid * (kMaxSeqs / kThreads) + i;
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const uint64_t y = (c ? x1 : x0) % per_head;
+                if (y >= from && y - from < work[i]) {
+                    uint32_t j, k;
+                    ds5idx::pb_locate(seq(b), G, y - from, snap, p.whole, j, k);
+                    s_cut[c][0] = b, s_cut[c][1] = j, s_cut[c][2] = k;
+                    if (c == 0) s_from = from;
+                }
+            }
+            from += work[i];
         }
     }
-    bad = __ballot(bad) != 0;
-    for (int e = 0; e < D / 64; e++) a.out[row + lane + 64 * e] = bad ? NAN : o[e] / l;
+    __syncthreads();
+    const bool last_wg = wg + 1 == n_wg;
+    const ds5idx::PbCut stop = last_wg ? ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0}
+                                       : ds5idx::PbCut{uniform((uint32_t)(x1 / per_head)), uniform(s_cut[1][0]),
+                                                       uniform(s_cut[1][1]), uniform(s_cut[1][2])};
+    ds5idx::PbCut at{uniform((uint32_t)(x0 / per_head)), uniform(s_cut[0][0]), uniform(s_cut[0][1]), uniform(s_cut[0][2])};
+
+    // where the tile begins on the line of work
+    uint64_t line = at.kvh * per_head + s_from + ds5idx::pb_before(useq(at.b), G, at.j);
+
+    const uint64_t slots = (uint64_t)bt.n_pages * bt.page_size;
+    A t;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        t.koff[i] = ds5idx::pb_load_off(D, false, i, lane);
+        t.voff[i] = ds5idx::pb_load_off(D, true, i, lane);
+    }
+    const float scale_log2 = p.a.scale * kLog2e;
+    bool head = false;  // this workgroup begins a tile that it does not end
+
+    bool at_end = false;
+    for (; !at_end && ds5idx::pb_next(at, stop, n_seqs, bt.n_kv_heads, G, useq, at_end); at.j++, at.k = 0) {
+        const uint32_t kvh = at.kvh, b = at.b;
+        const ds5idx::PbSeq sq = useq(b);
+        const uint32_t nt = ds5idx::pb_tiles(sq, G), ti = ds5idx::pb_tile_at(at.j, nt);
+        const ds5idx::PbTile tile = ds5idx::pb_tile(sq, G, ti);
+        const uint32_t end = at_end ? stop.k : tile.kv, kb = at.k, kv = tile.kv;
+        const uint32_t start = uniform(s_start[b]);
+        const bool poison = (uniform(s_before[b]) & kPoison) != 0;
+        const bool narrow = tile.rows <= (uint32_t)kNarrow;
+        const uint32_t rg = narrow ? 0 : wave & 3, kg = narrow ? wave : wave >> 2;
+        const f16* kpool = p.a.k_pool + (uint64_t)kvh * slots * D;
+        const f16* vpool = p.a.v_pool + (uint64_t)kvh * slots * D;
+        const uint64_t tb = (uint64_t)b * bt.max_pages;
+        const int32_t* table = bt.page_table;
+
+        if (tid == 0) s_bad = 0xffffffffu, s_odd = 0;
+        __syncthreads();
+        // ---- this wavefront's 32 query rows
+        const int r32 = lane & 31, h = lane >> 5;
+        const uint32_t row = tile.row0 + min(32 * rg + r32, tile.rows - 1);
+        t.lim = sq.before + row / G;
+        const uint32_t lim_lo = sq.before + (tile.row0 + min(32 * rg, tile.rows - 1)) / G;
+        const uint32_t lim_hi = sq.before + (tile.row0 + min(32 * rg + 31, tile.rows - 1)) / G;
+        {
+            const uint64_t from = ((uint64_t)(start + row / G) * bt.n_q_heads + kvh * G + row % G) * D;
+            if constexpr (Q16) {
+                t.fac = scale_log2;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) t.qh[ks] = *(const f16x8*)((const f16*)p.a.q + from + 16 * ks + 8 * h);
+            } else {
+                float4 q0[KS], q1[KS];
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const float* src = (const float*)p.a.q + from + 16 * ks + 8 * h;
+                    q0[ks] = *(const float4*)src;
+                    q1[ks] = *(const float4*)(src + 4);
+                }
+                // the row times a power of two that brings its largest element to 2^13 .. 2^14: the
+                // operands then hold 22 bits of it whatever its size
+                float big = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+                    big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(q0[ks].x), fabsf(q0[ks].y)), fmaxf(fabsf(q0[ks].z), fabsf(q0[ks].w))),
+                                           fmaxf(fmaxf(fabsf(q1[ks].x), fabsf(q1[ks].y)), fmaxf(fabsf(q1[ks].z), fabsf(q1[ks].w)))));
+                big = swap32_op(big, OpMax{});
+                const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 14 : 0;
+                t.fac = ldexpf(scale_log2, e);
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) {
+                    const float x[8] = {q0[ks].x, q0[ks].y, q0[ks].z, q0[ks].w, q1[ks].x, q1[ks].y, q1[ks].z, q1[ks].w};
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        f16x2 hi, lo;
+                        split2(ldexpf(x[i], -e), ldexpf(x[i + 1], -e), hi, lo);
+                        t.qh[ks][i] = hi[0], t.qh[ks][i + 1] = hi[1];
+                        t.ql[ks][i] = lo[0], t.ql[ks][i + 1] = lo[1];
+                    }
+                }
+            }
+        }
+        uint32_t bad = 0xffffffffu;  // the first position of a page out of range
+        // the pool row of a group of 16 positions (inside one page: page_size and pos are multiples of 16)
+        auto group_row = [&](uint32_t pos) -> uint64_t {
+            const int32_t pg = scalar_i32(table, tb + pos / bt.page_size);
+            const bool in = (uint32_t)pg < bt.n_pages;
+            if (!in) bad = min(bad, pos);
+            return (in ? (uint64_t)(uint32_t)pg * bt.page_size : 0) + pos % bt.page_size;
+        };
+        bool careful = false;
+        for (;;) {  // a second time, with infinities and NaN of V set aside, if the first left any in O
+            t.m = -INFINITY;
+            t.l = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) t.O[dt] = f32x16{};
+            bool odd = false;
+            auto one = [&](char* sk, char* sv, uint32_t key0) {
+                if (key0 + 32 > end) A::zero_tail(sv, key0, end, lane);
+                const bool mask = key0 + 31 > lim_lo || key0 + 32 > end;
+                if (careful || (key0 + 31 > lim_lo && lim_hi > lim_lo)) odd |= A::clean(sv, lane);
+                if (mask) t.template block<true>(sk, sv, key0, end, lane);
+                else t.template block<false>(sk, sv, key0, end, lane);
+            };
+            if (poison) {
+            } else if (narrow) {
+                // blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
+                // loaded once this one's scores stand, its V once this one's products do
+                char* const sk = s_kv + wave * 2 * HALF;
+                char* const sv = sk + HALF;
+                auto load = [&](uint32_t key0, const f16* pool, uint32_t lds, const uint32_t* off) {
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        const uint32_t pos = uniform(min(key0 + 16 * g, (end - 1) / 16 * 16));
+                        A::load_group(lds + g * (HALF / 2), pool + group_row(pos) * D, off);
+                    }
+                };
+                for (uint32_t key0 = kb + 32 * wave; key0 < end; key0 += 32 * kWaves) {
+                    load(key0, kpool, lds_addr(sk), t.koff);
+                    load(key0, vpool, lds_addr(sv), t.voff);
+                    wait_loads<0>();
+                    one(sk, sv, key0);
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                }
+            } else {
+                // steps of 128 positions for all: wavefront w loads rows 16 w .. of K and V, the next step's
+                // while this one is worked on; wavefronts 0 .. 3 take the first 64 of them, 4 .. 7 the others
+                const uint32_t steps = (end - kb + 127) / 128;
+                auto load = [&](uint32_t s) {
+                    const uint32_t pos = uniform(min(kb + 128 * s + 16 * wave, (end - 1) / 16 * 16));
+                    const uint64_t r = group_row(pos) * D;
+                    const uint32_t lds = lds_addr(s_kv) + (s & 1) * BUF + wave * 16 * RB;
+                    A::load_group(lds, kpool + r, t.koff);
+                    A::load_group(lds + BUF / 2, vpool + r, t.voff);
+                };
+                load(0);
+                wait_loads<0>();
+                __syncthreads();
+                for (uint32_t s = 0; s < steps; s++) {
+                    if (s + 1 < steps) load(s + 1);
+                    char* const buf = s_kv + (s & 1) * BUF;
+#pragma unroll 1
+                    for (uint32_t i = 0; i < 2; i++) {
+                        const uint32_t r0 = 64 * kg + 32 * i, key0 = kb + 128 * s + r0;
+                        if (key0 < end && key0 <= lim_hi && 32 * rg < tile.rows) one(buf + r0 * RB, buf + BUF / 2 + r0 * RB, key0);
+                    }
+                    wait_loads<0>();
+                    __syncthreads();
+                }
+            }
+            if (bad != 0xffffffffu && lane == 0) atomicMin(&s_bad, bad);
+            if (odd && lane == 0) s_odd = 1;
+            if (careful) break;
+            bool broken = false;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) broken = broken || !(fabsf(t.O[dt][e]) < INFINITY);
+            if (__syncthreads_or(broken) == 0) break;
+            careful = true;
+        }
+
+        // ---- the wavefronts' parts of the tile together: rows of O through LDS
+        const float l = swap32_op(t.l, OpAdd{});
+        __syncthreads();
+        {
+            char* area = s_kv + wave * 2 * HALF;
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t c = 8 * dt + 2 * i + h;
+                    *(float4*)(area + r32 * 4 * D + (c ^ (r32 & (A::CH - 1))) * 16) =
+                        float4{t.O[dt][4 * i], t.O[dt][4 * i + 1], t.O[dt][4 * i + 2], t.O[dt][4 * i + 3]};
+                }
+            if (h == 0) {
+                s_m[wave][r32] = t.m;
+                s_l[wave][r32] = l;
+            }
+        }
+        __syncthreads();
+        const bool done = kb == 0 && end == kv;
+        const bool begins = kb == 0 && end < kv;
+        const uint32_t slot = 2 * wg + (begins ? 1 : 0);
+        const bool any_odd = s_odd != 0;
+        const uint32_t bad_pos = s_bad;
+        for (uint32_t i = tid; i < tile.rows * A::CH; i += kThreads) {
+            const uint32_t rr = i / A::CH, c = i % A::CH, r = rr & 31;
+            const uint32_t w0 = narrow ? 0 : rr >> 5, wstep = narrow ? 1 : 4;
+            float M = -INFINITY, L = 0.0f;
+            for (uint32_t w = w0; w < (uint32_t)kWaves; w += wstep) M = fmaxf(M, s_m[w][r]);
+            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t w = w0; w < (uint32_t)kWaves; w += wstep) {
+                const float mw = s_m[w][r];
+                if (mw == -INFINITY) continue;  // it saw none of the row's positions
+                const float f = fast_exp2(mw - M);
+                L += s_l[w][r] * f;
+                o += *(const f32x4*)(s_kv + w * 2 * HALF + r * 4 * D + (c ^ (r & (A::CH - 1))) * 16) * f;
+            }
+            const uint32_t packed = tile.row0 + rr, pos = sq.before + packed / G;
+            if (any_odd)  // what was set aside, for the rows that attend it
+                for (uint32_t key = kb; key < end && key <= pos; key++) {
+                    const int32_t pg = table[tb + key / bt.page_size];
+                    if ((uint32_t)pg >= bt.n_pages) continue;
+                    const f16x4 v = *(const f16x4*)(vpool + ((uint64_t)(uint32_t)pg * bt.page_size + key % bt.page_size) * D + 4 * c);
+                    for (int e = 0; e < 4; e++)
+                        if (!(fabsf((float)v[e]) < INFINITY)) o[e] += (float)v[e];
+                }
+            if (poison || pos >= bad_pos) M = 0.0f, L = NAN;
+            if (done || poison) {
+                const uint64_t to = ((uint64_t)(start + packed / G) * bt.n_q_heads + kvh * G + packed % G) * D + 4 * c;
+                *(f32x4*)(p.a.out + to) = o / L;
+            } else {
+                *(f32x4*)(p.part_o + ((uint64_t)slot * kRows + rr) * D + 4 * c) = o;
+                if (c == 0) p.part_ml[(uint64_t)slot * kRows + rr] = float2{M, L};
+            }
+        }
+        if (begins && !poison) {
+            head = true;
+            if (tid == 0) {
+                // the last workgroup with a part of the tile: the last cut that is not within `snap` of its end
+                const uint64_t tile_end = line + ds5idx::pb_tile_work(sq, G, ti);
+                p.descs[wg] = MergeDesc{ds5idx::pb_last_cut(total, n_wg, tile_end - snap), tile.rows, tile.row0, kvh, start};
+            }
+        }
+        __syncthreads();  // LDS is free again
+        line += ds5idx::pb_tile_work(sq, G, ti);
+    }
+    if (!head && tid == 0 && p.descs) p.descs[wg].rows = 0;
+}
+
+// The parts of the tiles that several workgroups share, one tile per blockIdx.x: the head part of
+// workgroup w, then the parts of w + 1 .. last, folded in that order. 256 threads are D / 4 columns
+// and 1024 / D slots: with few parts a slot folds a row of its own, with many the slots share a
+// row's parts and join through LDS.
+template <int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnParams p) {
+    constexpr int CH = D / 4, SL = 256 / CH;
+    __shared__ f32x4 s_o[SL][CH];
+    __shared__ float2 s_ml[SL];
+    const MergeDesc d = p.descs[blockIdx.x];
+    if (d.rows == 0) return;
+    const uint32_t w = blockIdx.x, n = d.last - w + 1, G = p.group;
+    const uint32_t c = threadIdx.x % CH, sl = threadIdx.x / CH;
+    auto slot_of = [&](uint32_t i) -> uint64_t { return i == 0 ? 2 * w + 1 : 2 * (w + i); };
+    // parts first, first + step, ... of a row
+    auto fold = [&](uint32_t row, uint32_t first, uint32_t step, float& M, float& L, f32x4& o) {
+        constexpr int U = 4;
+        M = -INFINITY, L = 0.0f, o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t i0 = first; i0 < n; i0 += U * step) {
+            float2 ml[U];
+            f32x4 v[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const uint64_t s = slot_of(min(i0 + u * step, n - 1)) * kRows + row;
+                ml[u] = p.part_ml[s];
+                v[u] = *(const f32x4*)(p.part_o + s * D + 4 * c);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (i0 + u * step >= n || ml[u].x == -INFINITY) continue;
+                const float m = fmaxf(M, ml[u].x), fa = M == -INFINITY ? 0.0f : fast_exp2(M - m), fb = fast_exp2(ml[u].x - m);
+                L = L * fa + ml[u].y * fb;
+                o = o * fa + v[u] * fb;
+                M = m;
+            }
+        }
+    };
+    auto write = [&](uint32_t row, f32x4 o, float L) {
+        const uint32_t packed = d.row0 + row;
+        *(f32x4*)(p.a.out + ((uint64_t)(d.token0 + packed / G) * p.a.batch.n_q_heads + d.kvh * G + packed % G) * D + 4 * c) = o / L;
+    };
+    float M, L;
+    f32x4 o;
+    if (n <= 4) {
+        for (uint32_t row = blockIdx.y * SL + sl; row < d.rows; row += gridDim.y * SL) {
+            fold(row, 0, 1, M, L, o);
+            write(row, o, L);
+        }
+        return;
+    }
+    for (uint32_t row = blockIdx.y; row < d.rows; row += gridDim.y) {
+        fold(row, sl, SL, M, L, o);
+        __syncthreads();
+        s_o[sl][c] = o;
+        if (c == 0) s_ml[sl] = float2{M, L};
+        __syncthreads();
+        if (sl == 0) {
+            float mm = -INFINITY, ll = 0.0f;
+            for (int i = 0; i < SL; i++) mm = fmaxf(mm, s_ml[i].x);
+            f32x4 oo = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < SL; i++) {
+                if (s_ml[i].x == -INFINITY) continue;
+                const float f = fast_exp2(s_ml[i].x - mm);
+                ll += s_ml[i].y * f;
+                oo += s_o[i][c] * f;
+            }
+            write(row, oo, ll);
+        }
+    }
 }
 
 }  // namespace
@@ -207,15 +724,40 @@ int launch_paged_append(ds5_hip_ctx* ctx, const PagedAppendLaunch& a) {
 }
 
 int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
-    const uint64_t items = (uint64_t)a.batch.n_tokens * a.batch.n_q_heads;
-    const dim3 grid((uint32_t)((items + 3) / 4)), block(256);
-    const char* name = "paged_attention_kernel";
-    if (a.batch.head_dim == 128) {
-        if (a.q_f16) DS5_TIMED_LAUNCH(ctx, name, (paged_attention_kernel<128, true>), grid, block, 0, ctx->stream, a);
-        else DS5_TIMED_LAUNCH(ctx, name, (paged_attention_kernel<128, false>), grid, block, 0, ctx->stream, a);
-    } else {
-        if (a.q_f16) DS5_TIMED_LAUNCH(ctx, name, (paged_attention_kernel<64, true>), grid, block, 0, ctx->stream, a);
-        else DS5_TIMED_LAUNCH(ctx, name, (paged_attention_kernel<64, false>), grid, block, 0, ctx->stream, a);
+    const PagedBatch& b = a.batch;
+    AttnParams p{};
+    p.a = a;
+    p.group = b.n_q_heads / b.n_kv_heads;
+    const uint64_t rows = (uint64_t)b.n_tokens * p.group, tiles = rows / kRows + std::min<uint64_t>(b.n_seqs, b.n_tokens);
+    // the work that the plan counts, at most: below 2^54
+    if ((double)b.n_kv_heads * tiles * ((double)p.group * ((double)b.max_seq_len + kRows) + rows + kRows) >= 18014398509481984.0)
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "paged_attention: batch too large");
+    // Up to 256 positions a workgroup's eight wavefronts take a tile in one go: none is cut then,
+    // and nothing merged. (Nor without the context's memory for parts.)
+    p.whole = !ctx->split_buf || b.max_seq_len <= 256;
+    const uint64_t most = b.n_kv_heads * tiles * (p.whole ? 1 : ((uint64_t)b.max_seq_len + 2 * ds5idx::kPbUnit - 1) / (2 * ds5idx::kPbUnit));
+    const uint32_t cus = std::min(kMaxGrid, ctx->cu_count > 0 ? (uint32_t)ctx->cu_count : kMaxGrid);
+    const dim3 grid((uint32_t)std::min<uint64_t>(most, cus)), block(kThreads);
+    if (!p.whole) {
+        static_assert(2ull * kMaxGrid * kRows * 128 * sizeof(float) <= kSplitBytesMax, "parts fit the context's buffer");
+        static_assert(2ull * kMaxGrid * kRows * sizeof(float2) + kMaxGrid * sizeof(MergeDesc) <= kSplitStateBytes, "and their state");
+        p.part_o = (float*)ctx->split_buf;
+        p.part_ml = (float2*)((char*)ctx->split_buf + kSplitBytesMax);
+        p.descs = (MergeDesc*)(p.part_ml + 2ull * kMaxGrid * kRows);
     }
+    const char* name = "paged_attention_kernel";
+    if (b.head_dim == 128) {
+        if (a.q_f16) DS5_TIMED_LAUNCH(ctx, name, (paged_attention_kernel<128, true>), grid, block, 0, ctx->stream, p);
+        else DS5_TIMED_LAUNCH(ctx, name, (paged_attention_kernel<128, false>), grid, block, 0, ctx->stream, p);
+    } else {
+        if (a.q_f16) DS5_TIMED_LAUNCH(ctx, name, (paged_attention_kernel<64, true>), grid, block, 0, ctx->stream, p);
+        else DS5_TIMED_LAUNCH(ctx, name, (paged_attention_kernel<64, false>), grid, block, 0, ctx->stream, p);
+    }
+    if (int rc = ds5_after_launch(ctx, name)) return rc;
+    if (p.whole || grid.x == 1) return DS5_OK;  // one workgroup cuts nothing
+    const dim3 merge(grid.x, (uint32_t)std::min<uint64_t>(rows, 16));
+    name = "paged_merge_kernel";
+    if (b.head_dim == 128) DS5_TIMED_LAUNCH(ctx, name, paged_merge_kernel<128>, merge, dim3(256), 0, ctx->stream, p);
+    else DS5_TIMED_LAUNCH(ctx, name, paged_merge_kernel<64>, merge, dim3(256), 0, ctx->stream, p);
     return ds5_after_launch(ctx, name);
 }
