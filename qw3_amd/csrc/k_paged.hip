@@ -165,6 +165,7 @@ struct MergeDesc {
 struct AttnParams {
     PagedAttentionLaunch a;
     uint32_t group;
+    uint32_t page_shift;  // log2 of page_size where it is a power of two, else 0
     bool whole;        // no tile is cut
     float* part_o;     // [2 * workgroups, kRows, D]: slot 2 w the part that workgroup w continues, 2 w + 1 the one it begins
     float2* part_ml;   // [2 * workgroups, kRows]: reference and sum
@@ -183,6 +184,10 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 }
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+
+__device__ __forceinline__ uint64_t uniform64(uint64_t v) {
+    return ((uint64_t)uniform((uint32_t)(v >> 32)) << 32) | uniform((uint32_t)v);
+}
 
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // at most N vector-memory operations of the wavefront in flight
@@ -214,22 +219,72 @@ struct Attn {
     float fac;       // score = product * fac, log2 units
     float m, l;      // reference, this lane's part of the sum
     uint32_t lim;    // the row's last position
-    uint32_t koff[NB], voff[NB];
+    uint32_t koff, voff;  // lane's offsets of a row group's first load
 
-    // Loads the 16 rows from `row` of the pool (rows of RB bytes) into 16 * RB bytes of LDS.
-    __device__ __forceinline__ static void load_group(uint32_t lds, const f16* row, const uint32_t* off) {
+    // The lane's 8 elements of each k-step of its query row, at element `from` of q.
+    __device__ __forceinline__ void load_q(const AttnParams& p, uint64_t from) {
+        const float scale_log2 = p.a.scale * kLog2e;
+        if constexpr (Q16) {
+            fac = scale_log2;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) qh[ks] = *(const f16x8*)((const f16*)p.a.q + from + 16 * ks);
+        } else {
+            float4 q0[KS], q1[KS];
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const float* src = (const float*)p.a.q + from + 16 * ks;
+                q0[ks] = *(const float4*)src;
+                q1[ks] = *(const float4*)(src + 4);
+            }
+            // the row times a power of two that brings its largest element to 2^13 .. 2^14: the
+            // operands then hold 22 bits of it whatever its size
+            float big = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+                big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(q0[ks].x), fabsf(q0[ks].y)), fmaxf(fabsf(q0[ks].z), fabsf(q0[ks].w))),
+                                       fmaxf(fmaxf(fabsf(q1[ks].x), fabsf(q1[ks].y)), fmaxf(fabsf(q1[ks].z), fabsf(q1[ks].w)))));
+            big = swap32_op(big, OpMax{});
+            const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 14 : 0;
+            fac = ldexpf(scale_log2, e);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                const float x[8] = {q0[ks].x, q0[ks].y, q0[ks].z, q0[ks].w, q1[ks].x, q1[ks].y, q1[ks].z, q1[ks].w};
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    f16x2 hi, lo;
+                    split2(ldexpf(x[i], -e), ldexpf(x[i + 1], -e), hi, lo);
+                    qh[ks][i] = hi[0], qh[ks][i + 1] = hi[1];
+                    ql[ks][i] = lo[0], ql[ks][i + 1] = lo[1];
+                }
+            }
+        }
+    }
+
+    // Loads the 16 rows from `row` of the pool (rows of RB bytes) into 16 * RB bytes of LDS: a load's
+    // immediate offset counts for both addresses, and load b's lanes read `off` with bit 6 (b's own
+    // part of the K rows' swizzle) turned.
+    template <bool V>
+    __device__ __forceinline__ static void load_group(uint32_t lds, const f16* row, uint32_t off) {
         const uint64_t v = (uint64_t)row;
         const uint64_t base = ((uint64_t)uniform((uint32_t)(v >> 32)) << 32) | uniform((uint32_t)v);
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[b]), "s"(base),
-                         "s"(uniform(lds + 1024 * b))
+        const uint32_t o1 = V ? off : off ^ 64, o2 = V ? off : off ^ 128, o3 = V ? off : off ^ 192;
+        if constexpr (NB == 4)
+            asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
+                         "global_load_lds_dwordx4 %1, %4 offset:1024\n\tglobal_load_lds_dwordx4 %2, %4 offset:2048\n\t"
+                         "global_load_lds_dwordx4 %3, %4 offset:3072" ::"v"(off), "v"(o1), "v"(o2), "v"(o3), "s"(base),
+                         "s"(uniform(lds))
+                         : "m0", "memory");
+        else
+            asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\t"
+                         "global_load_lds_dwordx4 %1, %2 offset:1024" ::"v"(off), "v"(o1), "s"(base), "s"(uniform(lds))
                          : "m0", "memory");
     }
 
-    // One block of 32 positions from key0, its K and V rows in LDS: scores, weights, sums.
-    template <bool MASK>
-    __device__ __forceinline__ void block(const char* sk, const char* sv, uint32_t key0, uint32_t end, int lane) {
+    // One block of 32 positions from key0, its K and V rows in LDS: scores, weights, sums. scored():
+    // called when the scores stand (K is read), landed(): before V is read.
+    template <class Scored, class Landed>
+    __device__ __forceinline__ void block(const char* sk, const char* sv, uint32_t key0, uint32_t end, bool mask, int lane,
+                                          Scored scored, Landed landed) {
         const int r32 = lane & 31, h = lane >> 5, g16 = lane >> 4, i16 = lane & 15;
         f32x16 S;
         const char* krow = sk + r32 * RB;
@@ -241,11 +296,12 @@ struct Attn {
             else S = mfma_32x32x16(k, qh[ks], S);
             if constexpr (!Q16) S = mfma_32x32x16(k, ql[ks], S);
         }
+        scored();
         // lane (r32, h): score e is position key0 + 8 (e / 4) + 4 h + e % 4 of row r32
         float t[16];
 #pragma unroll
         for (int e = 0; e < 16; e++) t[e] = S[e] * fac;
-        if constexpr (MASK) {
+        if (mask) {  // uniform
             const int seen = (int)min(lim, end - 1) - (int)key0 - 4 * h;
 #pragma unroll
             for (int e = 0; e < 16; e++)
@@ -279,6 +335,7 @@ struct Attn {
             ph[e / 8][e % 8] = hi[0], ph[e / 8][e % 8 + 1] = hi[1];
             pl[e / 8][e % 8] = lo[0], pl[e / 8][e % 8 + 1] = lo[1];
         }
+        landed();
         // V^T operand of positions 16 s + [0, 16): the transpose read gives lane i of 16 column i
         // of 4 rows; element jj of the operand is position 16 s + 8 (jj / 4) + 4 h + jj % 4
         const char* vrow = sv + (4 * (g16 >> 1) + (i16 >> 2)) * RB;
@@ -321,6 +378,31 @@ struct Attn {
     }
 };
 
+// Infinities and NaN of V that were set aside, added to a row's 4 elements from 4 c: those of
+// positions begin .. end of sequence b. (Only where there are any.)
+__device__ __noinline__ f32x4 add_odd_values(const f16* vpool, const int32_t* table, uint32_t page_size, uint32_t n_pages, uint32_t D,
+                                             uint32_t begin, uint32_t end, uint32_t c, f32x4 o) {
+    for (uint32_t key = begin; key < end; key++) {
+        const int32_t pg = table[key / page_size];
+        if ((uint32_t)pg >= n_pages) continue;
+        const f16x4 v = *(const f16x4*)(vpool + ((uint64_t)(uint32_t)pg * page_size + key % page_size) * D + 4 * c);
+        for (int e = 0; e < 4; e++)
+            if (!(fabsf((float)v[e]) < INFINITY)) o[e] += (float)v[e];
+    }
+    return o;
+}
+
+// The workgroup's way along the batch's line of work, kept in LDS by thread 0; the piece it is at
+// is read back by all, so that the loops over positions hold nothing of it in registers.
+struct Walk {
+    ds5idx::PbCut at, stop;
+    uint64_t line, per_head, total;  // where the tile at `at` begins; one kv head's work, and all
+    uint32_t wg, n_wg;
+    uint32_t more, at_end;           // there is a piece; it is the last
+    ds5idx::PbTile tile;
+    uint32_t start, before, poison, begin, end;  // the sequence's first row, tokens before its rows; the piece's positions
+};
+
 template <int D, bool Q16>
 __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p) {
     using A = Attn<D, Q16>;
@@ -329,243 +411,231 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     __shared__ uint32_t s_start[kMaxSeqs], s_n[kMaxSeqs], s_before[kMaxSeqs];
     __shared__ float s_m[kWaves][32], s_l[kWaves][32];
     __shared__ uint64_t s_scan[kWaves];
-    __shared__ uint32_t s_cut[2][3];
-    __shared__ uint64_t s_from;
+    __shared__ Walk s_walk;
     __shared__ uint32_t s_bad, s_odd;
 
-    const PagedBatch& bt = p.a.batch;
-    const uint32_t tid = threadIdx.x, lane = tid & 63, G = p.group;
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = uniform(tid >> 6);
-    const uint32_t n_seqs = bt.n_seqs;
+    const uint32_t n_seqs = p.a.batch.n_seqs;
     constexpr uint32_t kPoison = 0x80000000u;  // in s_before: the sequence's rows are NaN
-
-    // ---- the batch's sequences and their work
-    uint64_t work[kMaxSeqs / kThreads];
-    uint64_t mine = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kMaxSeqs / kThreads; i++) {
-        const uint32_t b = tid * (kMaxSeqs / kThreads) + i;
-        work[i] = 0;
-        if (b < n_seqs) {
-            const int64_t s0 = bt.starts[b], s1 = bt.starts[b + 1], len = bt.seq_lens[b];
-            const int64_t c0 = max(s0, (int64_t)0), c1 = min(s1, (int64_t)bt.n_tokens);
-            const uint32_t n = c1 > c0 ? (uint32_t)(c1 - c0) : 0;
-            const bool ok = c0 == s0 && c1 == s1 && len >= s1 - s0 && len <= (int64_t)bt.max_seq_len;
-            s_start[b] = (uint32_t)c0;
-            s_n[b] = n;
-            s_before[b] = ok ? (uint32_t)(len - n) : kPoison;
-            if (n) work[i] = ds5idx::pb_seq_work(ds5idx::PbSeq{n, ok ? (uint32_t)(len - n) : 0u}, G);
-        }
-        mine += work[i];
-    }
     auto seq = [&](uint32_t b) { return ds5idx::PbSeq{s_n[b], s_before[b] & ~kPoison}; };
-    auto useq = [&](uint32_t b) { return ds5idx::PbSeq{uniform(s_n[b]), uniform(s_before[b]) & ~kPoison}; };
-    uint64_t upto = mine;  // inclusive over the wavefront
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up(upto, o, 64);
-        if ((int)lane >= o) upto += y;
-    }
-    if (lane == 63) s_scan[wave] = upto;
-    __syncthreads();
-    uint64_t base = 0, per_head = 0;
-    for (uint32_t w = 0; w < (uint32_t)kWaves; w++) {
-        base += w < wave ? s_scan[w] : 0;
-        per_head += s_scan[w];
-    }
-    const uint64_t total = per_head * bt.n_kv_heads;
-    const uint32_t grid = gridDim.x;
-    if (total == 0) {
-        if (tid == 0 && p.descs) p.descs[blockIdx.x].rows = 0;
-        return;
-    }
-    const uint32_t n_wg = p.whole ? grid : ds5idx::pb_workgroups(total, G, grid);
-    // A full grid's consecutive parts go to one XCD (workgroup i runs on XCD i % 8), so that a
-    // sequence's K and V come into few L2s.
-    const uint32_t wg = n_wg == grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
-    if (wg >= n_wg) {
-        if (tid == 0 && p.descs) p.descs[wg].rows = 0;
-        return;
-    }
-    const uint64_t snap = ds5idx::pb_snap(total, n_wg, G);
-    const uint64_t x0 = ds5idx::pb_cut_at(total, wg, n_wg), x1 = ds5idx::pb_cut_at(total, wg + 1, n_wg);
+
+    // ---- the batch's sequences and their work; this workgroup's part of it
     {
-        uint64_t from = base + upto - mine;
+        const PagedBatch& bt = p.a.batch;
+        const uint32_t G = p.group;
+        uint64_t work[kMaxSeqs / kThreads];
+        uint64_t mine = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kMaxSeqs / kThreads; i++) {
             const uint32_t b = tid * (kMaxSeqs / kThreads) + i;
+            work[i] = 0;
+            if (b < n_seqs) {
+                const int64_t s0 = bt.starts[b], s1 = bt.starts[b + 1], len = bt.seq_lens[b];
+                const int64_t c0 = max(s0, (int64_t)0), c1 = min(s1, (int64_t)bt.n_tokens);
+                const uint32_t n = c1 > c0 ? (uint32_t)(c1 - c0) : 0;
+                const bool ok = c0 == s0 && c1 == s1 && len >= s1 - s0 && len <= (int64_t)bt.max_seq_len;
+                s_start[b] = (uint32_t)c0;
+                s_n[b] = n;
+                s_before[b] = ok ? (uint32_t)(len - n) : kPoison;
+                if (n) work[i] = ds5idx::pb_seq_work(ds5idx::PbSeq{n, ok ? (uint32_t)(len - n) : 0u}, G);
+            }
+            mine += work[i];
+        }
+        uint64_t upto = mine;  // inclusive over the wavefront
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
-                const uint64_t y = (c ? x1 : x0) % per_head;
-                if (y >= from && y - from < work[i]) {
-                    uint32_t j, k;
-                    ds5idx::pb_locate(seq(b), G, y - from, snap, p.whole, j, k);
-                    s_cut[c][0] = b, s_cut[c][1] = j, s_cut[c][2] = k;
-                    if (c == 0) s_from = from;
-                }
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint64_t y = __shfl_up(upto, o, 64);
+            if ((int)lane >= o) upto += y;
+        }
+        if (lane == 63) s_scan[wave] = upto;
+        __syncthreads();
+        uint64_t from = upto - mine, per_head = 0;
+        for (uint32_t w = 0; w < (uint32_t)kWaves; w++) {
+            from += w < wave ? s_scan[w] : 0;
+            per_head += s_scan[w];
+        }
+        per_head = uniform64(per_head);
+        const uint64_t total = per_head * bt.n_kv_heads;
+        const uint32_t grid = gridDim.x;
+        const uint32_t n_wg = total == 0 ? 0 : p.whole ? grid : ds5idx::pb_workgroups(total, G, grid);
+        // A full grid's consecutive parts go to one XCD (workgroup i runs on XCD i % 8), so that a
+        // sequence's K and V come into few L2s.
+        const uint32_t wg = n_wg == grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
+        if (tid == 0 && p.descs) p.descs[wg].rows = 0;  // until it begins a tile that it does not end
+        if (wg >= n_wg) return;
+        const uint64_t snap = ds5idx::pb_snap(total, n_wg, G);
+        const uint64_t x0 = ds5idx::pb_cut_at(total, wg, n_wg), x1 = ds5idx::pb_cut_at(total, wg + 1, n_wg);
+        const uint32_t h0 = (uint32_t)(x0 / per_head), h1 = (uint32_t)(x1 / per_head);
+        const uint64_t y0 = x0 - h0 * per_head, y1 = x1 - h1 * per_head;
+        if (tid == 0) {
+            s_walk.per_head = per_head, s_walk.total = total;
+            s_walk.wg = wg, s_walk.n_wg = n_wg;
+            s_walk.at_end = 0;
+            if (wg + 1 == n_wg) s_walk.stop = ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0};
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kMaxSeqs / kThreads; i++) {
+            const uint32_t b = tid * (kMaxSeqs / kThreads) + i;
+            uint32_t j, k;
+            if (y0 >= from && y0 - from < work[i]) {
+                ds5idx::pb_locate(seq(b), G, y0 - from, snap, p.whole, j, k);
+                s_walk.at = ds5idx::PbCut{h0, b, j, k};
+                s_walk.line = h0 * per_head + from + ds5idx::pb_before(seq(b), G, j);
+            }
+            if (wg + 1 < n_wg && y1 >= from && y1 - from < work[i]) {
+                ds5idx::pb_locate(seq(b), G, y1 - from, snap, p.whole, j, k);
+                s_walk.stop = ds5idx::PbCut{h1, b, j, k};
             }
             from += work[i];
         }
     }
     __syncthreads();
-    const bool last_wg = wg + 1 == n_wg;
-    const ds5idx::PbCut stop = last_wg ? ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0}
-                                       : ds5idx::PbCut{uniform((uint32_t)(x1 / per_head)), uniform(s_cut[1][0]),
-                                                       uniform(s_cut[1][1]), uniform(s_cut[1][2])};
-    ds5idx::PbCut at{uniform((uint32_t)(x0 / per_head)), uniform(s_cut[0][0]), uniform(s_cut[0][1]), uniform(s_cut[0][2])};
 
-    // where the tile begins on the line of work
-    uint64_t line = at.kvh * per_head + s_from + ds5idx::pb_before(useq(at.b), G, at.j);
-
-    const uint64_t slots = (uint64_t)bt.n_pages * bt.page_size;
     A t;
-#pragma unroll
-    for (int i = 0; i < NB; i++) {
-        t.koff[i] = ds5idx::pb_load_off(D, false, i, lane);
-        t.voff[i] = ds5idx::pb_load_off(D, true, i, lane);
-    }
-    const float scale_log2 = p.a.scale * kLog2e;
-    bool head = false;  // this workgroup begins a tile that it does not end
+    t.koff = ds5idx::pb_load_off(D, false, 0, lane);
+    t.voff = ds5idx::pb_load_off(D, true, 0, lane);
 
-    bool at_end = false;
-    for (; !at_end && ds5idx::pb_next(at, stop, n_seqs, bt.n_kv_heads, G, useq, at_end); at.j++, at.k = 0) {
-        const uint32_t kvh = at.kvh, b = at.b;
-        const ds5idx::PbSeq sq = useq(b);
-        const uint32_t nt = ds5idx::pb_tiles(sq, G), ti = ds5idx::pb_tile_at(at.j, nt);
-        const ds5idx::PbTile tile = ds5idx::pb_tile(sq, G, ti);
-        const uint32_t end = at_end ? stop.k : tile.kv, kb = at.k, kv = tile.kv;
-        const uint32_t start = uniform(s_start[b]);
-        const bool poison = (uniform(s_before[b]) & kPoison) != 0;
-        const bool narrow = tile.rows <= (uint32_t)kNarrow;
-        const uint32_t rg = narrow ? 0 : wave & 3, kg = narrow ? wave : wave >> 2;
-        const f16* kpool = p.a.k_pool + (uint64_t)kvh * slots * D;
-        const f16* vpool = p.a.v_pool + (uint64_t)kvh * slots * D;
-        const uint64_t tb = (uint64_t)b * bt.max_pages;
-        const int32_t* table = bt.page_table;
-
-        if (tid == 0) s_bad = 0xffffffffu, s_odd = 0;
-        __syncthreads();
-        // ---- this wavefront's 32 query rows
-        const int r32 = lane & 31, h = lane >> 5;
-        const uint32_t row = tile.row0 + min(32 * rg + r32, tile.rows - 1);
-        t.lim = sq.before + row / G;
-        const uint32_t lim_lo = sq.before + (tile.row0 + min(32 * rg, tile.rows - 1)) / G;
-        const uint32_t lim_hi = sq.before + (tile.row0 + min(32 * rg + 31, tile.rows - 1)) / G;
-        {
-            const uint64_t from = ((uint64_t)(start + row / G) * bt.n_q_heads + kvh * G + row % G) * D;
-            if constexpr (Q16) {
-                t.fac = scale_log2;
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++) t.qh[ks] = *(const f16x8*)((const f16*)p.a.q + from + 16 * ks + 8 * h);
-            } else {
-                float4 q0[KS], q1[KS];
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    const float* src = (const float*)p.a.q + from + 16 * ks + 8 * h;
-                    q0[ks] = *(const float4*)src;
-                    q1[ks] = *(const float4*)(src + 4);
-                }
-                // the row times a power of two that brings its largest element to 2^13 .. 2^14: the
-                // operands then hold 22 bits of it whatever its size
-                float big = 0.0f;
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++)
-                    big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(q0[ks].x), fabsf(q0[ks].y)), fmaxf(fabsf(q0[ks].z), fabsf(q0[ks].w))),
-                                           fmaxf(fmaxf(fabsf(q1[ks].x), fabsf(q1[ks].y)), fmaxf(fabsf(q1[ks].z), fabsf(q1[ks].w)))));
-                big = swap32_op(big, OpMax{});
-                const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 14 : 0;
-                t.fac = ldexpf(scale_log2, e);
-#pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    const float x[8] = {q0[ks].x, q0[ks].y, q0[ks].z, q0[ks].w, q1[ks].x, q1[ks].y, q1[ks].z, q1[ks].w};
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2) {
-                        f16x2 hi, lo;
-                        split2(ldexpf(x[i], -e), ldexpf(x[i + 1], -e), hi, lo);
-                        t.qh[ks][i] = hi[0], t.qh[ks][i + 1] = hi[1];
-                        t.ql[ks][i] = lo[0], t.ql[ks][i + 1] = lo[1];
-                    }
-                }
+    for (bool last_piece = false; !last_piece;) {
+        if (tid == 0) {
+            Walk& w = s_walk;
+            bool at_end = false;
+            w.more = ds5idx::pb_next(w.at, w.stop, n_seqs, p.a.batch.n_kv_heads, p.group, seq, at_end);
+            if (w.more) {
+                const ds5idx::PbSeq sq = seq(w.at.b);
+                w.tile = ds5idx::pb_tile(sq, p.group, ds5idx::pb_tile_at(w.at.j, ds5idx::pb_tiles(sq, p.group)));
+                w.start = s_start[w.at.b];
+                w.before = sq.before;
+                w.poison = s_before[w.at.b] & kPoison;
+                w.begin = w.at.k;
+                w.end = at_end ? w.stop.k : w.tile.kv;
+                w.at_end = at_end;
             }
+            s_bad = 0xffffffffu, s_odd = 0;
         }
-        uint32_t bad = 0xffffffffu;  // the first position of a page out of range
-        // the pool row of a group of 16 positions (inside one page: page_size and pos are multiples of 16)
-        auto group_row = [&](uint32_t pos) -> uint64_t {
-            const int32_t pg = scalar_i32(table, tb + pos / bt.page_size);
-            const bool in = (uint32_t)pg < bt.n_pages;
-            if (!in) bad = min(bad, pos);
-            return (in ? (uint64_t)(uint32_t)pg * bt.page_size : 0) + pos % bt.page_size;
-        };
-        bool careful = false;
-        for (;;) {  // a second time, with infinities and NaN of V set aside, if the first left any in O
-            t.m = -INFINITY;
-            t.l = 0.0f;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) t.O[dt] = f32x16{};
-            bool odd = false;
-            auto one = [&](char* sk, char* sv, uint32_t key0) {
-                if (key0 + 32 > end) A::zero_tail(sv, key0, end, lane);
-                const bool mask = key0 + 31 > lim_lo || key0 + 32 > end;
-                if (careful || (key0 + 31 > lim_lo && lim_hi > lim_lo)) odd |= A::clean(sv, lane);
-                if (mask) t.template block<true>(sk, sv, key0, end, lane);
-                else t.template block<false>(sk, sv, key0, end, lane);
+        __syncthreads();
+        if (uniform(s_walk.more) == 0) return;
+        last_piece = uniform(s_walk.at_end) != 0;
+        const bool narrow = uniform(s_walk.tile.rows) <= (uint32_t)kNarrow;
+        const int r32 = lane & 31, h = lane >> 5;
+        {
+            const uint32_t kb = uniform(s_walk.begin), end = uniform(s_walk.end);
+            const uint32_t rows = uniform(s_walk.tile.rows), row0 = uniform(s_walk.tile.row0), before = uniform(s_walk.before);
+            const uint32_t kvh = uniform(s_walk.at.kvh), b = uniform(s_walk.at.b), G = p.group;
+            const bool poison = uniform(s_walk.poison) != 0;
+            const uint32_t rg = narrow ? 0 : wave & 3;
+            const PagedBatch& bt = p.a.batch;
+            // ---- this wavefront's 32 query rows
+            const uint32_t row = row0 + min(32 * rg + r32, rows - 1);
+            t.lim = before + row / G;
+            const uint32_t lim_lo = uniform(before + (row0 + min(32 * rg, rows - 1)) / G);
+            const uint32_t lim_hi = uniform(before + (row0 + min(32 * rg + 31, rows - 1)) / G);
+            t.load_q(p, ((uint64_t)(uniform(s_walk.start) + row / G) * bt.n_q_heads + kvh * G + row % G) * D + 8 * h);
+
+            const uint64_t head = (uint64_t)kvh * bt.n_pages * bt.page_size * D;
+            const f16* const kpool = p.a.k_pool + head;
+            const f16* const vpool = p.a.v_pool + head;
+            const int32_t* const table = bt.page_table + (uint64_t)b * bt.max_pages;
+            uint32_t bad = 0xffffffffu;  // the first position of a page out of range
+            // the pool row of a group of 16 positions (inside one page: page_size and pos are multiples of 16)
+            auto group_row = [&](uint32_t pos) -> uint64_t {
+                const uint32_t page = p.page_shift ? pos >> p.page_shift : pos / bt.page_size;
+                const uint32_t pg = uniform((uint32_t)scalar_i32(table, page));
+                const bool in = pg < bt.n_pages;
+                if (!in) bad = min(bad, pos);
+                return ((in ? (uint64_t)pg * bt.page_size : 0) + (pos - page * bt.page_size)) * D;
             };
-            if (poison) {
-            } else if (narrow) {
-                // blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
-                // loaded once this one's scores stand, its V once this one's products do
-                char* const sk = s_kv + wave * 2 * HALF;
-                char* const sv = sk + HALF;
-                auto load = [&](uint32_t key0, const f16* pool, uint32_t lds, const uint32_t* off) {
+            const uint32_t last = (end - 1) / 16 * 16;  // a group of positions past the end re-reads the last one
+            bool careful = false;
+            for (;;) {  // a second time, with infinities and NaN of V set aside, if the first left any in O
+                t.m = -INFINITY;
+                t.l = 0.0f;
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        const uint32_t pos = uniform(min(key0 + 16 * g, (end - 1) / 16 * 16));
-                        A::load_group(lds + g * (HALF / 2), pool + group_row(pos) * D, off);
+                for (int dt = 0; dt < DT; dt++) t.O[dt] = f32x16{};
+                bool odd = false;
+                auto one = [&](char* sk, char* sv, uint32_t key0, auto scored, auto landed) {
+                    const bool mask = key0 + 31 > lim_lo || key0 + 32 > end;
+                    t.block(sk, sv, key0, end, mask, lane, scored, [&]() {
+                        landed();
+                        if (mask || careful) {
+                            if (key0 + 32 > end) A::zero_tail(sv, key0, end, lane);
+                            if (careful || lim_hi > lim_lo) odd |= A::clean(sv, lane);
+                        }
+                    });
+                };
+                if (poison) {
+                } else if (narrow) {
+                    // blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
+                    // loaded once this one's scores stand, its V once this one's products do
+                    char* const sk = s_kv + wave * 2 * HALF;
+                    char* const sv = sk + HALF;
+                    auto load_k = [&](uint32_t key0) {
+                        for (int g = 0; g < 2; g++)
+                            A::template load_group<false>(lds_addr(sk) + g * (HALF / 2), kpool + group_row(min(key0 + 16 * g, last)), t.koff);
+                    };
+                    auto load_v = [&](uint32_t key0) {
+                        for (int g = 0; g < 2; g++)
+                            A::template load_group<true>(lds_addr(sv) + g * (HALF / 2), vpool + group_row(min(key0 + 16 * g, last)), t.voff);
+                    };
+                    uint32_t key0 = kb + 32 * wave;
+                    if (key0 < end) {
+                        load_k(key0);
+                        load_v(key0);
                     }
-                };
-                for (uint32_t key0 = kb + 32 * wave; key0 < end; key0 += 32 * kWaves) {
-                    load(key0, kpool, lds_addr(sk), t.koff);
-                    load(key0, vpool, lds_addr(sv), t.voff);
-                    wait_loads<0>();
-                    one(sk, sv, key0);
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                }
-            } else {
-                // steps of 128 positions for all: wavefront w loads rows 16 w .. of K and V, the next step's
-                // while this one is worked on; wavefronts 0 .. 3 take the first 64 of them, 4 .. 7 the others
-                const uint32_t steps = (end - kb + 127) / 128;
-                auto load = [&](uint32_t s) {
-                    const uint32_t pos = uniform(min(kb + 128 * s + 16 * wave, (end - 1) / 16 * 16));
-                    const uint64_t r = group_row(pos) * D;
-                    const uint32_t lds = lds_addr(s_kv) + (s & 1) * BUF + wave * 16 * RB;
-                    A::load_group(lds, kpool + r, t.koff);
-                    A::load_group(lds + BUF / 2, vpool + r, t.voff);
-                };
-                load(0);
-                wait_loads<0>();
-                __syncthreads();
-                for (uint32_t s = 0; s < steps; s++) {
-                    if (s + 1 < steps) load(s + 1);
-                    char* const buf = s_kv + (s & 1) * BUF;
 #pragma unroll 1
-                    for (uint32_t i = 0; i < 2; i++) {
-                        const uint32_t r0 = 64 * kg + 32 * i, key0 = kb + 128 * s + r0;
-                        if (key0 < end && key0 <= lim_hi && 32 * rg < tile.rows) one(buf + r0 * RB, buf + BUF / 2 + r0 * RB, key0);
+                    for (; key0 < end; key0 += 32 * kWaves) {
+                        const uint32_t next = key0 + 32 * kWaves;
+                        wait_loads<2 * NB>();  // K is here; V may not be
+                        one(sk, sv, key0,
+                            [&]() {
+                                if (next < end) load_k(next);
+                            },
+                            [&]() {
+                                if (next < end) wait_loads<2 * NB>();
+                                else wait_loads<0>();
+                            });
+                        if (next < end) {
+                            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                            load_v(next);
+                        }
                     }
+                } else {
+                    // steps of 128 positions for all: wavefront w loads rows 16 w .. of K and V, the next step's
+                    // while this one is worked on; wavefronts 0 .. 3 take the first 64 of them, 4 .. 7 the others
+                    auto load = [&](uint32_t key0, uint32_t parity) {
+                        const uint64_t r = group_row(min(key0 + 16 * wave, last));
+                        const uint32_t lds = lds_addr(s_kv) + parity * BUF + wave * 16 * RB;
+                        A::template load_group<false>(lds, kpool + r, t.koff);
+                        A::template load_group<true>(lds + BUF / 2, vpool + r, t.voff);
+                    };
+                    load(kb, 0);
                     wait_loads<0>();
                     __syncthreads();
+                    uint32_t parity = 0;
+#pragma unroll 1
+                    for (uint32_t s0 = kb; s0 < end; s0 += 128, parity ^= 1) {
+                        if (s0 + 128 < end) load(s0 + 128, parity ^ 1);
+#pragma unroll 1
+                        for (uint32_t r0 = 64 * (wave >> 2); r0 < 64 * (wave >> 2) + 64; r0 += 32) {
+                            char* const sk = s_kv + parity * BUF + r0 * RB;
+                            if (s0 + r0 < end && s0 + r0 <= lim_hi && 32 * rg < rows)
+                                one(sk, sk + BUF / 2, s0 + r0, []() {}, []() {});
+                        }
+                        wait_loads<0>();
+                        __syncthreads();
+                    }
                 }
+                if (bad != 0xffffffffu && lane == 0) atomicMin(&s_bad, bad);
+                if (odd && lane == 0) s_odd = 1;
+                if (careful) break;
+                bool broken = false;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) broken = broken || !(fabsf(t.O[dt][e]) < INFINITY);
+                if (__syncthreads_or(broken) == 0) break;
+                careful = true;
             }
-            if (bad != 0xffffffffu && lane == 0) atomicMin(&s_bad, bad);
-            if (odd && lane == 0) s_odd = 1;
-            if (careful) break;
-            bool broken = false;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) broken = broken || !(fabsf(t.O[dt][e]) < INFINITY);
-            if (__syncthreads_or(broken) == 0) break;
-            careful = true;
         }
 
         // ---- the wavefronts' parts of the tile together: rows of O through LDS
@@ -587,12 +657,15 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             }
         }
         __syncthreads();
-        const bool done = kb == 0 && end == kv;
-        const bool begins = kb == 0 && end < kv;
+        const uint32_t kb = uniform(s_walk.begin), end = uniform(s_walk.end), wg = uniform(s_walk.wg), G = p.group;
+        const uint32_t row0 = uniform(s_walk.tile.row0), rows = uniform(s_walk.tile.rows), before = uniform(s_walk.before);
+        const uint32_t start = uniform(s_walk.start), kvh = uniform(s_walk.at.kvh);
+        const bool done = kb == 0 && end == uniform(s_walk.tile.kv), poison = uniform(s_walk.poison) != 0;
+        const bool begins = kb == 0 && !done;
         const uint32_t slot = 2 * wg + (begins ? 1 : 0);
-        const bool any_odd = s_odd != 0;
-        const uint32_t bad_pos = s_bad;
-        for (uint32_t i = tid; i < tile.rows * A::CH; i += kThreads) {
+        const bool any_odd = uniform(s_odd) != 0;
+        const uint32_t bad_pos = uniform(s_bad);
+        for (uint32_t i = tid; i < rows * A::CH; i += kThreads) {
             const uint32_t rr = i / A::CH, c = i % A::CH, r = rr & 31;
             const uint32_t w0 = narrow ? 0 : rr >> 5, wstep = narrow ? 1 : 4;
             float M = -INFINITY, L = 0.0f;
@@ -605,36 +678,36 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                 L += s_l[w][r] * f;
                 o += *(const f32x4*)(s_kv + w * 2 * HALF + r * 4 * D + (c ^ (r & (A::CH - 1))) * 16) * f;
             }
-            const uint32_t packed = tile.row0 + rr, pos = sq.before + packed / G;
-            if (any_odd)  // what was set aside, for the rows that attend it
-                for (uint32_t key = kb; key < end && key <= pos; key++) {
-                    const int32_t pg = table[tb + key / bt.page_size];
-                    if ((uint32_t)pg >= bt.n_pages) continue;
-                    const f16x4 v = *(const f16x4*)(vpool + ((uint64_t)(uint32_t)pg * bt.page_size + key % bt.page_size) * D + 4 * c);
-                    for (int e = 0; e < 4; e++)
-                        if (!(fabsf((float)v[e]) < INFINITY)) o[e] += (float)v[e];
-                }
+            const uint32_t packed = row0 + rr, pos = before + packed / G;
+            if (any_odd) {
+                const PagedBatch& bt = p.a.batch;
+                o = add_odd_values(p.a.v_pool + (uint64_t)kvh * bt.n_pages * bt.page_size * D, bt.page_table + (uint64_t)s_walk.at.b * bt.max_pages,
+                                   bt.page_size, bt.n_pages, D, kb, min(end, pos + 1), c, o);
+            }
             if (poison || pos >= bad_pos) M = 0.0f, L = NAN;
             if (done || poison) {
-                const uint64_t to = ((uint64_t)(start + packed / G) * bt.n_q_heads + kvh * G + packed % G) * D + 4 * c;
+                const uint64_t to = ((uint64_t)(start + packed / G) * p.a.batch.n_q_heads + kvh * G + packed % G) * D + 4 * c;
                 *(f32x4*)(p.a.out + to) = o / L;
             } else {
                 *(f32x4*)(p.part_o + ((uint64_t)slot * kRows + rr) * D + 4 * c) = o;
                 if (c == 0) p.part_ml[(uint64_t)slot * kRows + rr] = float2{M, L};
             }
         }
-        if (begins && !poison) {
-            head = true;
-            if (tid == 0) {
-                // the last workgroup with a part of the tile: the last cut that is not within `snap` of its end
-                const uint64_t tile_end = line + ds5idx::pb_tile_work(sq, G, ti);
-                p.descs[wg] = MergeDesc{ds5idx::pb_last_cut(total, n_wg, tile_end - snap), tile.rows, tile.row0, kvh, start};
-            }
-        }
         __syncthreads();  // LDS is free again
-        line += ds5idx::pb_tile_work(sq, G, ti);
+        if (tid == 0) {
+            Walk& w = s_walk;
+            const ds5idx::PbSeq sq = seq(w.at.b);
+            const uint64_t tile_end =
+                w.line + ds5idx::pb_tile_work(sq, G, ds5idx::pb_tile_at(w.at.j, ds5idx::pb_tiles(sq, G)));
+            // the last workgroup with a part of the tile: the last cut that is not within `snap` of its end
+            if (begins && !poison)
+                p.descs[wg] = MergeDesc{ds5idx::pb_last_cut(w.total, w.n_wg, tile_end - ds5idx::pb_snap(w.total, w.n_wg, G)), rows,
+                                        row0, kvh, start};
+            w.line = tile_end;
+            w.at.j++;
+            w.at.k = 0;
+        }
     }
-    if (!head && tid == 0 && p.descs) p.descs[wg].rows = 0;
 }
 
 // The parts of the tiles that several workgroups share, one tile per blockIdx.x: the head part of
@@ -728,6 +801,7 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     AttnParams p{};
     p.a = a;
     p.group = b.n_q_heads / b.n_kv_heads;
+    p.page_shift = (b.page_size & (b.page_size - 1)) == 0 ? (uint32_t)__builtin_ctz(b.page_size) : 0;
     const uint64_t rows = (uint64_t)b.n_tokens * p.group, tiles = rows / kRows + std::min<uint64_t>(b.n_seqs, b.n_tokens);
     // the work that the plan counts, at most: below 2^54
     if ((double)b.n_kv_heads * tiles * ((double)p.group * ((double)b.max_seq_len + kRows) + rows + kRows) >= 18014398509481984.0)
