@@ -4,6 +4,8 @@
 // The pool is that of k_decode.hip's paged decode: f16 [n_kv_heads, n_pages * page_size, D],
 // position p of sequence b in slot page_table[b][p / page_size] * page_size + p % page_size.
 // Sequence b holds the batch's rows starts[b] .. starts[b + 1] - 1, its newest tokens.
+#include <type_traits>
+
 #include "ds5_common.hpp"
 
 namespace {
@@ -151,6 +153,7 @@ constexpr int kThreads = 512, kWaves = 8;
 constexpr int kRows = ds5idx::kPbRows, kNarrow = ds5idx::kPbNarrow;
 constexpr uint32_t kMaxSeqs = DS5_PAGED_MAX_SEQS;
 constexpr uint32_t kMaxGrid = 256;
+constexpr uint32_t kWindow = 1024;  // page table entries in LDS at a time
 // Weights are exp2(score - reference): the reference starts 2^8 below the row's maximum and moves
 // when a weight would pass 2^15, so that in f16 hi + lo a weight keeps its 22 bits down to 2^-22
 // of the largest and counts down to 2^-33 of it.
@@ -185,6 +188,13 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 
+// The same value, worked out anew where it is used: the compiler otherwise keeps what follows from it in
+// registers across the loops, and spills.
+__device__ __forceinline__ uint32_t here(uint32_t v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
     return ((uint64_t)uniform((uint32_t)(v >> 32)) << 32) | uniform((uint32_t)v);
 }
@@ -199,10 +209,27 @@ __device__ __forceinline__ void split2(float x0, float x1, f16x2& hi, f16x2& lo)
     hi = f16x2{(f16)x0, (f16)x1};
     lo = f16x2{(f16)(x0 - (float)hi[0]), (f16)(x1 - (float)hi[1])};
 }
+// The same of two weights (at least 0), both halves rounded towards 0 (one packed conversion each and
+// a mixed-precision fma per residual): 21 bits, 2^-22 too small in the mean.
+__device__ __forceinline__ void split2_weights(float x0, float x1, f16x2& hi, f16x2& lo) {
+    hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+    lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi[0], -1.0f, x0),
+                                                              __builtin_fmaf((float)hi[1], -1.0f, x1)));
+}
 
-// A scalar load of one i32 (the scalar cache holds nothing of before the launch).
-__device__ __forceinline__ int32_t scalar_i32(const int32_t* p, uint64_t i) {
-    return ((const __attribute__((address_space(4))) int32_t*)p)[i];
+// The largest of a block's 16 scores on both lanes of a row. max3 as asm takes the products as they are
+// (compiled from fmaxf each operand is canonicalised first); the first maximum is compiled, so that it
+// waits for the products' result, and the others depend on it.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float row_max(const f32x16& S) {
+    float a = fmaxf(S[0], S[15]);
+#pragma unroll
+    for (int e = 1; e < 15; e += 2) a = max3(a, S[e], S[e + 1]);
+    return swap32_op(a, OpMax{});
 }
 
 template <int D, bool Q16>
@@ -210,8 +237,7 @@ struct Attn {
     static constexpr int KS = D / 16, DT = D / 32, RB = 2 * D;
     static constexpr int NB = 16 * RB / 1024;      // direct-to-LDS loads of a group of 16 rows
     static constexpr int HALF = 32 * RB;           // bytes of 32 rows
-    static constexpr int BUF = 2 * kRows * RB;     // wide: K then V of 128 positions
-    static constexpr int AREA = kWaves * 2 * HALF; // = 2 * BUF
+    static constexpr int AREA = kWaves * 2 * HALF; // K and V of a block for each wavefront, or four stages of two blocks
     static constexpr int CH = D / 4;               // float4 of an O row
 
     f32x16 O[DT];
@@ -221,13 +247,33 @@ struct Attn {
     uint32_t lim;    // the row's last position
     uint32_t koff, voff;  // lane's offsets of a row group's first load
 
+    // Loads the 8 rows from `row` (half a group) into 8 * RB bytes of LDS.
+    template <bool V>
+    __device__ __forceinline__ static void load_half(uint32_t lds, const f16* row, uint32_t off) {
+        const uint64_t base = uniform64((uint64_t)row);
+        const uint32_t o1 = V ? off : off ^ 64;
+        if constexpr (NB == 4)
+            asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\t"
+                         "global_load_lds_dwordx4 %1, %2 offset:1024" ::"v"(off), "v"(o1), "s"(base), "s"(uniform(lds))
+                         : "m0", "memory");
+        else
+            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(uniform(lds))
+                         : "m0", "memory");
+    }
+
     // The lane's 8 elements of each k-step of its query row, at element `from` of q.
     __device__ __forceinline__ void load_q(const AttnParams& p, uint64_t from) {
-        const float scale_log2 = p.a.scale * kLog2e;
+        // fac stays above 0 (a negative scale goes into the row's sign), so that the largest product is
+        // the largest score and -inf stays -inf
+        const bool minus = p.a.scale < 0.0f;
+        const float scale_log2 = fmaxf(fabsf(p.a.scale * kLog2e), 1e-37f);
         if constexpr (Q16) {
             fac = scale_log2;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) qh[ks] = *(const f16x8*)((const f16*)p.a.q + from + 16 * ks);
+            for (int ks = 0; ks < KS; ks++) {
+                qh[ks] = *(const f16x8*)((const f16*)p.a.q + from + 16 * ks);
+                if (minus) qh[ks] = -qh[ks];
+            }
         } else {
             float4 q0[KS], q1[KS];
 #pragma unroll
@@ -245,14 +291,15 @@ struct Attn {
                                        fmaxf(fmaxf(fabsf(q1[ks].x), fabsf(q1[ks].y)), fmaxf(fabsf(q1[ks].z), fabsf(q1[ks].w)))));
             big = swap32_op(big, OpMax{});
             const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 14 : 0;
-            fac = ldexpf(scale_log2, e);
+            fac = fmaxf(ldexpf(scale_log2, e), 1e-37f);
+            const float unit = minus ? -1.0f : 1.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
                 const float x[8] = {q0[ks].x, q0[ks].y, q0[ks].z, q0[ks].w, q1[ks].x, q1[ks].y, q1[ks].z, q1[ks].w};
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     f16x2 hi, lo;
-                    split2(ldexpf(x[i], -e), ldexpf(x[i + 1], -e), hi, lo);
+                    split2(ldexpf(x[i] * unit, -e), ldexpf(x[i + 1] * unit, -e), hi, lo);
                     qh[ks][i] = hi[0], qh[ks][i + 1] = hi[1];
                     ql[ks][i] = lo[0], ql[ks][i + 1] = lo[1];
                 }
@@ -265,8 +312,7 @@ struct Attn {
     // part of the K rows' swizzle) turned.
     template <bool V>
     __device__ __forceinline__ static void load_group(uint32_t lds, const f16* row, uint32_t off) {
-        const uint64_t v = (uint64_t)row;
-        const uint64_t base = ((uint64_t)uniform((uint32_t)(v >> 32)) << 32) | uniform((uint32_t)v);
+        const uint64_t base = uniform64((uint64_t)row);
         const uint32_t o1 = V ? off : off ^ 64, o2 = V ? off : off ^ 128, o3 = V ? off : off ^ 192;
         if constexpr (NB == 4)
             asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
@@ -280,38 +326,49 @@ struct Attn {
                          : "m0", "memory");
     }
 
-    // One block of 32 positions from key0, its K and V rows in LDS: scores, weights, sums. scored():
-    // called when the scores stand (K is read), landed(): before V is read.
-    template <class Scored, class Landed>
-    __device__ __forceinline__ void block(const char* sk, const char* sv, uint32_t key0, uint32_t end, bool mask, int lane,
-                                          Scored scored, Landed landed) {
-        const int r32 = lane & 31, h = lane >> 5, g16 = lane >> 4, i16 = lane & 15;
-        f32x16 S;
-        const char* krow = sk + r32 * RB;
-        const uint32_t kx = (ds5idx::pb_swz(D, false, r32) ^ h) * 16;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const f16x8 k = *(const f16x8*)(krow + (kx ^ (32 * ks)));
-            if (ks == 0) S = mfma_32x32x16(k, qh[0], f32x16{});
-            else S = mfma_32x32x16(k, qh[ks], S);
-            if constexpr (!Q16) S = mfma_32x32x16(k, ql[ks], S);
+    // A block is 32 positions; its products' operands come from LDS:
+    //   S^T [32 positions x 32 rows] = K . Q^T     O^T [D x 32 rows] += V^T . P^T    v_mfma_f32_32x32x16_f16
+    // With S transposed a lane (r32, h) holds 16 scores of query row r32, score e that of position
+    // 8 (e / 4) + 4 h + e % 4, and the P^T operand is the lane's own weights.
+    struct Lane {
+        uint32_t k, v;  // byte offsets of the lane's operands: the block's K row r32, V rows of the transpose read
+        __device__ __forceinline__ explicit Lane(uint32_t lane) {
+            const uint32_t r32 = lane & 31, h = lane >> 5, i16 = lane & 15, g16 = lane >> 4;
+            k = r32 * RB + (ds5idx::pb_swz(D, false, r32) ^ h) * 16;
+            v = (4 * h + (i16 >> 2)) * RB +
+                ((2 * (g16 & 1) + ((i16 & 3) >> 1)) ^ ds5idx::pb_swz(D, true, i16 >> 2)) * 16 + 8 * (i16 & 1);
         }
-        scored();
-        // lane (r32, h): score e is position key0 + 8 (e / 4) + 4 h + e % 4 of row r32
-        float t[16];
+    };
+    // (a row's chunks are RB bytes aligned to RB, so xor in its low bits stays in the row)
+    __device__ __forceinline__ static f16x8 kread(const char* sk, const Lane& ln, int ks) {
+        return *(const f16x8*)(sk + (ln.k ^ (32 * ks)));
+    }
+    // positions 16 s + [0, 16): the transpose read gives lane i of 16 column i of 4 rows; element jj of the
+    // operand is position 16 s + 8 (jj / 4) + 4 h + jj % 4, as the weights lie
+    __device__ __forceinline__ static f16x8 vread(const char* sv, const Lane& ln, int s, int dt) {
+        const char* at = sv + (ln.v ^ (64 * dt)) + 16 * s * RB;
+        const f16x4 a = lds_read_tr16(at), b = lds_read_tr16(at + 8 * RB);
+        return f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+    __device__ __forceinline__ void product(f32x16& S, const f16x8& k, int ks) const {
+        S = mfma_32x32x16(k, qh[ks], S);
+        if constexpr (!Q16) S = mfma_32x32x16(k, ql[ks], S);
+    }
+    __device__ __forceinline__ void scores(f32x16& S, const char* sk, const Lane& ln) const {
+        S = f32x16{};
 #pragma unroll
-        for (int e = 0; e < 16; e++) t[e] = S[e] * fac;
-        if (mask) {  // uniform
-            const int seen = (int)min(lim, end - 1) - (int)key0 - 4 * h;
+        for (int ks = 0; ks < KS; ks++) product(S, kread(sk, ln, ks), ks);
+    }
+    __device__ __forceinline__ void mask_scores(f32x16& S, uint32_t key0, uint32_t end, uint32_t h) const {
+        const int seen = (int)min(lim, end - 1) - (int)key0 - 4 * (int)h;
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-                if (8 * (e / 4) + e % 4 > seen) t[e] = -INFINITY;
-        }
-        float mx = t[0];
-#pragma unroll
-        for (int e = 1; e < 16; e++) mx = fmaxf(mx, t[e]);
-        mx = swap32_op(mx, OpMax{});
-        if (__ballot(mx > m + kMove) != 0) {  // (m is -inf before the row's first score)
+        for (int e = 0; e < 16; e++)
+            if (8 * (e / 4) + e % 4 > seen) S[e] = -INFINITY;
+    }
+    // Moves the reference where a score (the row's largest: mx, before fac) asks for it.
+    __device__ __forceinline__ void rescale(float mx) {
+        mx *= fac;
+        if (__builtin_expect(__ballot(mx > m + kMove) != 0, 0)) {  // (m is -inf before the row's first score)
             const float m_new = mx > m + kMove ? mx - kHead : m;
             const float alpha = m_new == m ? 1.0f : fast_exp2(m - m_new);
             l *= alpha;
@@ -319,50 +376,113 @@ struct Attn {
             for (int dt = 0; dt < DT; dt++) O[dt] *= alpha;
             m = m_new;
         }
-        const float ref = m == -INFINITY ? 0.0f : m;  // a row that has seen nothing: weights exp2(-inf)
-        float p[16];
-#pragma unroll
-        for (int e = 0; e < 16; e++) p[e] = fast_exp2(t[e] - ref);
+    }
+    // The reference to subtract: 0 for a row that has seen nothing (its weights are exp2(-inf)).
+    __device__ __forceinline__ float reference() const { return m == -INFINITY ? 0.0f : m; }
+
+    // One block by itself. scored(): called when the scores stand (K is read), landed(): before V is read.
+    template <class Scored, class Landed>
+    __device__ __forceinline__ void block(const char* sk, const char* sv, uint32_t key0, uint32_t end, bool mask, Lane ln,
+                                          uint32_t h, Scored scored, Landed landed) {
+        f32x16 S;
+        ln.k = here(ln.k), ln.v = here(ln.v);
+        scores(S, sk, ln);
+        scored();
+        if (mask) mask_scores(S, key0, end, h);  // uniform
+        rescale(row_max(S));
+        const float ref = reference();
         float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) sum += (p[e] + p[e + 1]) + (p[e + 2] + p[e + 3]);
-        l += sum;
         f16x8 ph[2], pl[2];
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
+            const float p0 = fast_exp2(__builtin_fmaf(S[e], fac, -ref)), p1 = fast_exp2(__builtin_fmaf(S[e + 1], fac, -ref));
+            sum += p0 + p1;
             f16x2 hi, lo;
-            split2(p[e], p[e + 1], hi, lo);
+            split2_weights(p0, p1, hi, lo);
             ph[e / 8][e % 8] = hi[0], ph[e / 8][e % 8 + 1] = hi[1];
             pl[e / 8][e % 8] = lo[0], pl[e / 8][e % 8 + 1] = lo[1];
         }
+        l += sum;
         landed();
-        // V^T operand of positions 16 s + [0, 16): the transpose read gives lane i of 16 column i
-        // of 4 rows; element jj of the operand is position 16 s + 8 (jj / 4) + 4 h + jj % 4
-        const char* vrow = sv + (4 * (g16 >> 1) + (i16 >> 2)) * RB;
-        const uint32_t vx = (2 * (g16 & 1) + ((i16 & 3) >> 1)) * 16 + 8 * (i16 & 1) + 16 * ds5idx::pb_swz(D, true, i16 >> 2);
 #pragma unroll
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
-                const f16x4 a = lds_read_tr16(vrow + 16 * s * RB + (vx ^ (64 * dt)));
-                const f16x4 b = lds_read_tr16(vrow + (16 * s + 8) * RB + (vx ^ (64 * dt)));
-                const f16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+                const f16x8 v = vread(sv, ln, s, dt);
                 O[dt] = mfma_32x32x16(v, ph[s], O[dt]);
                 O[dt] = mfma_32x32x16(v, pl[s], O[dt]);
             }
     }
 
+    // One block of a run of them: its scores S (largest mx) stand already; the products of the next block's
+    // (K at sk; after the last block whatever lies there, its scores dropped) go beside the weights of S, the products with V beside the other half of the
+    // weights and the next scores' maximum. load_k(), load_v(): later rows' loads, issued between products,
+    // where the wait for the load path to take them costs nothing. LDS reads run kAhead operands ahead of their products. The
+    // scheduling fences keep this order: a product occupies the matrix core for 32 cycles, in which the
+    // wavefront issues the VALU work beside it.
+    template <class LoadK, class LoadV>
+    __device__ __forceinline__ void step(f32x16& S, float& mx, const char* sk, const char* sv, Lane ln, LoadK load_k, LoadV load_v) {
+        ln.k = here(ln.k), ln.v = here(ln.v);
+        constexpr int kAhead = 3, NV = 2 * DT, E0 = 8 / KS, E1 = 8 / DT;
+        rescale(mx);
+        const float ref = reference();
+        f16x8 ph[2], pl[2], kop[KS], vop[NV];
+        float w[2], sum = 0.0f;
+        auto weight = [&](int e) {
+            w[e % 2] = fast_exp2(__builtin_fmaf(S[e], fac, -ref));
+            sum += w[e % 2];
+            if (e % 2) {
+                f16x2 hi, lo;
+                split2_weights(w[0], w[1], hi, lo);
+                ph[e / 8][e % 8 - 1] = hi[0], ph[e / 8][e % 8] = hi[1];
+                pl[e / 8][e % 8 - 1] = lo[0], pl[e / 8][e % 8] = lo[1];
+                if (e % 8 == 7) asm volatile("" : "+v"(ph[e / 8]), "+v"(pl[e / 8]));  // here, not where they are used
+            }
+        };
+        f32x16 Sn = f32x16{};
+#pragma unroll
+        for (int n = 0; n < kAhead; n++) kop[n] = kread(sk, ln, n);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < KS; n++) {
+            if (n + kAhead < KS) kop[n + kAhead] = kread(sk, ln, n + kAhead);
+            else vop[n + kAhead - KS] = vread(sv, ln, (n + kAhead - KS) / DT, (n + kAhead - KS) % DT);
+            product(Sn, kop[n], n);
+            if (n == 1) load_k();
+            if (n == KS - 1) load_v();
+#pragma unroll
+            for (int e = 0; e < E0; e++) weight(E0 * n + e);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int n = 0; n < NV; n++) {
+            if (n + kAhead < NV) vop[n + kAhead] = vread(sv, ln, (n + kAhead) / DT, (n + kAhead) % DT);
+            O[n % DT] = mfma_32x32x16(vop[n], ph[n / DT], O[n % DT]);
+            O[n % DT] = mfma_32x32x16(vop[n], pl[n / DT], O[n % DT]);
+            if (n < DT) {
+#pragma unroll
+                for (int e = 0; e < E1; e++) weight(8 + E1 * n + e);
+            }
+            if (n == NV - 2) mx = row_max(Sn);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        l += sum;
+        S = Sn;
+    }
+
     // V rows of a block from position `end` on to zero (their weights are 0, what they hold may be
     // anything), and with CLEAN every infinity and NaN: true if there was one. The wavefronts that
     // share the rows write the same values.
-    __device__ __forceinline__ static void zero_tail(char* sv, uint32_t key0, uint32_t end, int lane) {
-        for (int c = lane; c < 32 * RB / 16; c += 64)
+    __device__ __forceinline__ static void zero_tail(char* sv, uint32_t key0, uint32_t end, uint32_t lane) {
+#pragma unroll 1
+        for (uint32_t c = here(lane); c < 32 * RB / 16; c += 64)
             if (key0 + c / (RB / 16) >= end) *(u32x4*)(sv + 16 * c) = u32x4{0u, 0u, 0u, 0u};
         __builtin_amdgcn_wave_barrier();
     }
-    __device__ __forceinline__ static bool clean(char* sv, int lane) {
+    __device__ __forceinline__ static bool clean(char* sv, uint32_t lane) {
         bool found = false;
-        for (int c = lane; c < 32 * RB / 16; c += 64) {
+#pragma unroll 1
+        for (uint32_t c = here(lane); c < 32 * RB / 16; c += 64) {
             u32x4 v = *(const u32x4*)(sv + 16 * c);
             bool odd = false;
 #pragma unroll
@@ -406,13 +526,14 @@ struct Walk {
 template <int D, bool Q16>
 __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p) {
     using A = Attn<D, Q16>;
-    constexpr int KS = A::KS, DT = A::DT, RB = A::RB, NB = A::NB, HALF = A::HALF, BUF = A::BUF;
+    constexpr int DT = A::DT, RB = A::RB, NB = A::NB, HALF = A::HALF;
     __shared__ __attribute__((aligned(1024))) char s_kv[A::AREA];
     __shared__ uint32_t s_start[kMaxSeqs], s_n[kMaxSeqs], s_before[kMaxSeqs];
     __shared__ float s_m[kWaves][32], s_l[kWaves][32];
     __shared__ uint64_t s_scan[kWaves];
     __shared__ Walk s_walk;
-    __shared__ uint32_t s_bad, s_odd;
+    __shared__ uint32_t s_bad, s_odd, s_broken;
+    __shared__ uint32_t s_pages[kWindow];  // the page table's entries of a window of the piece
 
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = uniform(tid >> 6);
@@ -492,10 +613,6 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     }
     __syncthreads();
 
-    A t;
-    t.koff = ds5idx::pb_load_off(D, false, 0, lane);
-    t.voff = ds5idx::pb_load_off(D, true, 0, lane);
-
     for (bool last_piece = false; !last_piece;) {
         if (tid == 0) {
             Walk& w = s_walk;
@@ -511,18 +628,27 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                 w.end = at_end ? w.stop.k : w.tile.kv;
                 w.at_end = at_end;
             }
-            s_bad = 0xffffffffu, s_odd = 0;
+            s_bad = 0xffffffffu, s_odd = s_broken = 0;
         }
         __syncthreads();
-        if (uniform(s_walk.more) == 0) return;
-        last_piece = uniform(s_walk.at_end) != 0;
-        const bool narrow = uniform(s_walk.tile.rows) <= (uint32_t)kNarrow;
-        const int r32 = lane & 31, h = lane >> 5;
+        const Walk& wk = *(const Walk*)((const char*)&s_walk + here(0));
+        if (uniform(wk.more) == 0) return;
+        last_piece = uniform(wk.at_end) != 0;
+        // The piece, in a form of its own for tiles of at most kNarrow rows (in one form of both the compiler
+        // spills: the accumulators then meet where the forms part and join).
+        auto piece = [&](auto form) {
+        constexpr bool narrow = decltype(form)::value;
+        const uint32_t tid = here(threadIdx.x), lane = tid & 63;
+        const uint32_t r32 = lane & 31, h = lane >> 5;
+        A t;
+        t.koff = ds5idx::pb_load_off(D, false, 0, lane);
+        t.voff = ds5idx::pb_load_off(D, true, 0, lane);
         {
-            const uint32_t kb = uniform(s_walk.begin), end = uniform(s_walk.end);
-            const uint32_t rows = uniform(s_walk.tile.rows), row0 = uniform(s_walk.tile.row0), before = uniform(s_walk.before);
-            const uint32_t kvh = uniform(s_walk.at.kvh), b = uniform(s_walk.at.b), G = p.group;
-            const bool poison = uniform(s_walk.poison) != 0;
+            const typename A::Lane ln(lane);
+            const uint32_t kb = uniform(wk.begin), end = uniform(wk.end);
+            const uint32_t rows = uniform(wk.tile.rows), row0 = uniform(wk.tile.row0), before = uniform(wk.before);
+            const uint32_t kvh = uniform(wk.at.kvh), b = uniform(wk.at.b), G = p.group;
+            const bool poison = uniform(wk.poison) != 0;
             const uint32_t rg = narrow ? 0 : wave & 3;
             const PagedBatch& bt = p.a.batch;
             // ---- this wavefront's 32 query rows
@@ -530,22 +656,14 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             t.lim = before + row / G;
             const uint32_t lim_lo = uniform(before + (row0 + min(32 * rg, rows - 1)) / G);
             const uint32_t lim_hi = uniform(before + (row0 + min(32 * rg + 31, rows - 1)) / G);
-            t.load_q(p, ((uint64_t)(uniform(s_walk.start) + row / G) * bt.n_q_heads + kvh * G + row % G) * D + 8 * h);
+            t.load_q(p, ((uint64_t)(uniform(wk.start) + row / G) * bt.n_q_heads + kvh * G + row % G) * D + 8 * h);
 
             const uint64_t head = (uint64_t)kvh * bt.n_pages * bt.page_size * D;
             const f16* const kpool = p.a.k_pool + head;
             const f16* const vpool = p.a.v_pool + head;
             const int32_t* const table = bt.page_table + (uint64_t)b * bt.max_pages;
-            uint32_t bad = 0xffffffffu;  // the first position of a page out of range
-            // the pool row of a group of 16 positions (inside one page: page_size and pos are multiples of 16)
-            auto group_row = [&](uint32_t pos) -> uint64_t {
-                const uint32_t page = p.page_shift ? pos >> p.page_shift : pos / bt.page_size;
-                const uint32_t pg = uniform((uint32_t)scalar_i32(table, page));
-                const bool in = pg < bt.n_pages;
-                if (!in) bad = min(bad, pos);
-                return ((in ? (uint64_t)pg * bt.page_size : 0) + (pos - page * bt.page_size)) * D;
-            };
-            const uint32_t last = (end - 1) / 16 * 16;  // a group of positions past the end re-reads the last one
+            const uint32_t page_size = bt.page_size, shift = p.page_shift;
+            auto page_of = [&](uint32_t pos) { return shift ? pos >> shift : pos / page_size; };
             bool careful = false;
             for (;;) {  // a second time, with infinities and NaN of V set aside, if the first left any in O
                 t.m = -INFINITY;
@@ -553,95 +671,141 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) t.O[dt] = f32x16{};
                 bool odd = false;
-                auto one = [&](char* sk, char* sv, uint32_t key0, auto scored, auto landed) {
-                    const bool mask = key0 + 31 > lim_lo || key0 + 32 > end;
-                    t.block(sk, sv, key0, end, mask, lane, scored, [&]() {
-                        landed();
-                        if (mask || careful) {
-                            if (key0 + 32 > end) A::zero_tail(sv, key0, end, lane);
-                            if (careful || lim_hi > lim_lo) odd |= A::clean(sv, lane);
-                        }
-                    });
+                auto masked = [&](uint32_t key0) { return key0 + 31 > lim_lo || key0 + 32 > end; };
+                auto clean = [&](char* sv, uint32_t key0) {  // V rows that some row of the tile does not attend
+                    if (key0 + 32 > end) A::zero_tail(sv, key0, end, lane);
+                    if (careful || lim_hi > lim_lo) odd |= A::clean(sv, lane);
                 };
-                if (poison) {
-                } else if (narrow) {
-                    // blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
-                    // loaded once this one's scores stand, its V once this one's products do
-                    char* const sk = s_kv + wave * 2 * HALF;
-                    char* const sv = sk + HALF;
-                    auto load_k = [&](uint32_t key0) {
-                        for (int g = 0; g < 2; g++)
-                            A::template load_group<false>(lds_addr(sk) + g * (HALF / 2), kpool + group_row(min(key0 + 16 * g, last)), t.koff);
-                    };
-                    auto load_v = [&](uint32_t key0) {
-                        for (int g = 0; g < 2; g++)
-                            A::template load_group<true>(lds_addr(sv) + g * (HALF / 2), vpool + group_row(min(key0 + 16 * g, last)), t.voff);
-                    };
-                    uint32_t key0 = kb + 32 * wave;
-                    if (key0 < end) {
-                        load_k(key0);
-                        load_v(key0);
+                // the piece in windows of kWindow pages (most pieces are one)
+                for (uint32_t from = poison ? end : kb, to; from < end; from = to) {
+                    const uint32_t page0 = uniform(page_of(from));
+                    const uint64_t window = ((uint64_t)page0 + kWindow) * page_size;
+                    to = window < end ? (uint32_t)window / 64 * 64 : end;
+                    if (from > kb) __syncthreads();  // everyone is done with the window before
+                    for (uint32_t i = tid; i <= page_of(to - 1) - page0; i += kThreads) {
+                        const uint32_t pg = (uint32_t)table[page0 + i];
+                        s_pages[i] = pg;
+                        if (pg >= bt.n_pages) atomicMin(&s_bad, max(from, (page0 + i) * page_size));
                     }
-#pragma unroll 1
-                    for (; key0 < end; key0 += 32 * kWaves) {
-                        const uint32_t next = key0 + 32 * kWaves;
-                        wait_loads<2 * NB>();  // K is here; V may not be
-                        one(sk, sv, key0,
-                            [&]() {
-                                if (next < end) load_k(next);
-                            },
-                            [&]() {
-                                if (next < end) wait_loads<2 * NB>();
-                                else wait_loads<0>();
-                            });
-                        if (next < end) {
-                            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                            load_v(next);
-                        }
-                    }
-                } else {
-                    // steps of 128 positions for all: wavefront w loads rows 16 w .. of K and V, the next step's
-                    // while this one is worked on; wavefronts 0 .. 3 take the first 64 of them, 4 .. 7 the others
-                    auto load = [&](uint32_t key0, uint32_t parity) {
-                        const uint64_t r = group_row(min(key0 + 16 * wave, last));
-                        const uint32_t lds = lds_addr(s_kv) + parity * BUF + wave * 16 * RB;
-                        A::template load_group<false>(lds, kpool + r, t.koff);
-                        A::template load_group<true>(lds + BUF / 2, vpool + r, t.voff);
-                    };
-                    load(kb, 0);
-                    wait_loads<0>();
                     __syncthreads();
-                    uint32_t parity = 0;
+                    // element offset of the pool row of pos, a multiple of 8 (a page out of range: page 0, and the
+                    // rows that attend it are NaN)
+                    auto row_of = [&](uint32_t pos) -> uint64_t {
+                        const uint32_t page = page_of(pos), pg = uniform(s_pages[page - page0]);
+                        return ((uint64_t)(pg < bt.n_pages ? pg : 0) * page_size + (pos - page * page_size)) * D;
+                    };
+                    if constexpr (narrow) {
+                        // blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
+                        // loaded once this one's scores stand, its V once this one's products do
+                        char* const sk = s_kv + wave * 2 * HALF;
+                        char* const sv = sk + HALF;
+                        const uint32_t last = (to - 1) / 16 * 16;  // a group of positions past the end re-reads the last one
+                        uint64_t r0, r1;
+                        auto rows_at = [&](uint32_t key0) { r0 = row_of(min(key0, last)), r1 = row_of(min(key0 + 16, last)); };
+                        auto load_k = [&]() {
+                            A::template load_group<false>(lds_addr(sk), kpool + r0, t.koff);
+                            A::template load_group<false>(lds_addr(sk) + HALF / 2, kpool + r1, t.koff);
+                        };
+                        auto load_v = [&]() {
+                            A::template load_group<true>(lds_addr(sv), vpool + r0, t.voff);
+                            A::template load_group<true>(lds_addr(sv) + HALF / 2, vpool + r1, t.voff);
+                        };
+                        uint32_t key0 = from + 32 * wave;
+                        if (key0 < to) {
+                            rows_at(key0);
+                            load_k();
+                            load_v();
+                        }
 #pragma unroll 1
-                    for (uint32_t s0 = kb; s0 < end; s0 += 128, parity ^= 1) {
-                        if (s0 + 128 < end) load(s0 + 128, parity ^ 1);
+                        for (; key0 < to; key0 += 32 * kWaves) {
+                            const uint32_t next = key0 + 32 * kWaves;
+                            const bool mask = masked(key0);
+                            rows_at(next);
+                            wait_loads<2 * NB>();  // K is here; V may not be
+                            t.block(sk, sv, key0, end, mask, ln, h,
+                                    [&]() {
+                                        if (next < to) load_k();
+                                    },
+                                    [&]() {
+                                        if (next < to) wait_loads<2 * NB>();
+                                        else wait_loads<0>();
+                                        if (mask || careful) clean(sv, key0);
+                                    });
+                            if (next < to) {
+                                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                                load_v();
+                            }
+                        }
+                    } else {
+                        // Steps of 64 positions through a ring of four stages of K and V: wavefront w loads rows
+                        // 8 w .. 8 w + 7, three steps ahead, into the stage that everyone left before the last
+                        // barrier; wavefronts 0 .. 3 take the first block of a step, 4 .. 7 the second. A step's K
+                        // and V have landed one step before their block (its scores are formed a block ahead).
+                        constexpr uint32_t STAGE = 2 * 64 * RB;
+                        const uint32_t steps = (to - from + 63) / 64, mine = 32 * (wave >> 2), last = (to - 1) / 8 * 8;
+                        const uint32_t koff = t.koff ^ (wave & 1) * (RB / 2);  // the K rows' swizzle of rows 8 .. 15 of 16
+                        auto row_at = [&](uint32_t i) { return row_of(min(from + 64 * i + 8 * wave, last)); };
+                        auto lds_at = [&](uint32_t i) -> uint32_t { return lds_addr(s_kv) + (i & 3) * STAGE + 8 * wave * RB; };
+                        auto k_of = [&](uint32_t i) -> char* { return s_kv + (i & 3) * STAGE + mine * RB; };
+                        // this wavefront's blocks: the first of the steps whose block holds a position its rows attend
+                        const uint32_t upto = min(to, lim_hi + 1), first = from + mine;
+                        const uint32_t blocks = 32 * rg < rows && upto > first ? (upto - first + 63) / 64 : 0;
+                        for (uint32_t i = 0; i < 3; i++) {  // (steps past the last re-read its rows)
+                            const uint64_t r = row_at(i);
+                            A::template load_half<false>(lds_at(i), kpool + r, koff);
+                            A::template load_half<true>(lds_at(i) + STAGE / 2, vpool + r, t.voff);
+                        }
+                        wait_loads<NB>();
+                        __syncthreads();
+                        f32x16 S;
+                        float mx = -INFINITY;
+                        if (blocks) {
+                            t.scores(S, k_of(0), ln);
+                            mx = row_max(S);
+                        }
 #pragma unroll 1
-                        for (uint32_t r0 = 64 * (wave >> 2); r0 < 64 * (wave >> 2) + 64; r0 += 32) {
-                            char* const sk = s_kv + parity * BUF + r0 * RB;
-                            if (s0 + r0 < end && s0 + r0 <= lim_hi && 32 * rg < rows)
-                                one(sk, sk + BUF / 2, s0 + r0, []() {}, []() {});
+                        for (uint32_t i = 0; i < steps; i++) {
+                            const uint64_t r = row_at(i + 3);
+                            auto load_k = [&]() { A::template load_half<false>(lds_at(i + 3), kpool + r, koff); };
+                            auto load_v = [&]() { A::template load_half<true>(lds_at(i + 3) + STAGE / 2, vpool + r, t.voff); };
+                            if (i < blocks) {
+                                const uint32_t key0 = first + 64 * i;
+                                char* const sv = k_of(i) + STAGE / 2;
+                                if (careful || masked(key0)) {
+                                    if (masked(key0)) {
+                                        t.mask_scores(S, key0, end, h);
+                                        mx = row_max(S);
+                                    }
+                                    clean(sv, key0);
+                                }
+                                t.step(S, mx, k_of(i + 1), sv, ln, load_k, load_v);
+                            } else {
+                                load_k();
+                                load_v();
+                            }
+                            wait_loads<NB>();
+                            __syncthreads();
                         }
                         wait_loads<0>();
-                        __syncthreads();
                     }
                 }
-                if (bad != 0xffffffffu && lane == 0) atomicMin(&s_bad, bad);
                 if (odd && lane == 0) s_odd = 1;
-                if (careful) break;
-                bool broken = false;
+                float zero = 0.0f;  // (NaN where O holds an infinity or NaN)
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) broken = broken || !(fabsf(t.O[dt][e]) < INFINITY);
-                if (__syncthreads_or(broken) == 0) break;
+                    for (int e = 0; e < 16; e++) zero = __builtin_fmaf(t.O[dt][e], 0.0f, zero);
+                if (__ballot(!(zero == 0.0f)) != 0 && lane == 0) s_broken = 1;
+                __syncthreads();
+                if (careful || uniform(s_broken) == 0) break;
                 careful = true;
             }
         }
 
         // ---- the wavefronts' parts of the tile together: rows of O through LDS
         const float l = swap32_op(t.l, OpAdd{});
-        __syncthreads();
         {
+            const uint32_t lane = here(tid) & 63, r32 = lane & 31, h = lane >> 5;
             char* area = s_kv + wave * 2 * HALF;
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
@@ -657,40 +821,60 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             }
         }
         __syncthreads();
-        const uint32_t kb = uniform(s_walk.begin), end = uniform(s_walk.end), wg = uniform(s_walk.wg), G = p.group;
-        const uint32_t row0 = uniform(s_walk.tile.row0), rows = uniform(s_walk.tile.rows), before = uniform(s_walk.before);
-        const uint32_t start = uniform(s_walk.start), kvh = uniform(s_walk.at.kvh);
-        const bool done = kb == 0 && end == uniform(s_walk.tile.kv), poison = uniform(s_walk.poison) != 0;
+        const uint32_t kb = uniform(wk.begin), end = uniform(wk.end), wg = uniform(wk.wg), G = p.group;
+        const uint32_t row0 = uniform(wk.tile.row0), rows = uniform(wk.tile.rows), before = uniform(wk.before);
+        const uint32_t start = uniform(wk.start), kvh = uniform(wk.at.kvh);
+        const bool done = kb == 0 && end == uniform(wk.tile.kv), poison = uniform(wk.poison) != 0;
         const bool begins = kb == 0 && !done;
         const uint32_t slot = 2 * wg + (begins ? 1 : 0);
         const bool any_odd = uniform(s_odd) != 0;
         const uint32_t bad_pos = uniform(s_bad);
-        for (uint32_t i = tid; i < rows * A::CH; i += kThreads) {
-            const uint32_t rr = i / A::CH, c = i % A::CH, r = rr & 31;
-            const uint32_t w0 = narrow ? 0 : rr >> 5, wstep = narrow ? 1 : 4;
-            float M = -INFINITY, L = 0.0f;
-            for (uint32_t w = w0; w < (uint32_t)kWaves; w += wstep) M = fmaxf(M, s_m[w][r]);
-            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (uint32_t w = w0; w < (uint32_t)kWaves; w += wstep) {
-                const float mw = s_m[w][r];
-                if (mw == -INFINITY) continue;  // it saw none of the row's positions
-                const float f = fast_exp2(mw - M);
-                L += s_l[w][r] * f;
-                o += *(const f32x4*)(s_kv + w * 2 * HALF + r * 4 * D + (c ^ (r & (A::CH - 1))) * 16) * f;
-            }
-            const uint32_t packed = row0 + rr, pos = before + packed / G;
-            if (any_odd) {
-                const PagedBatch& bt = p.a.batch;
-                o = add_odd_values(p.a.v_pool + (uint64_t)kvh * bt.n_pages * bt.page_size * D, bt.page_table + (uint64_t)s_walk.at.b * bt.max_pages,
-                                   bt.page_size, bt.n_pages, D, kb, min(end, pos + 1), c, o);
-            }
-            if (poison || pos >= bad_pos) M = 0.0f, L = NAN;
-            if (done || poison) {
-                const uint64_t to = ((uint64_t)(start + packed / G) * p.a.batch.n_q_heads + kvh * G + packed % G) * D + 4 * c;
-                *(f32x4*)(p.a.out + to) = o / L;
-            } else {
-                *(f32x4*)(p.part_o + ((uint64_t)slot * kRows + rr) * D + 4 * c) = o;
-                if (c == 0) p.part_ml[(uint64_t)slot * kRows + rr] = float2{M, L};
+        {
+            // a row's D / 4 columns to as many threads, kThreads / CH rows at a time
+            constexpr uint32_t CH = A::CH, PER = kThreads / CH;
+            const uint32_t c = here(tid) % CH, stride = narrow ? 2 * HALF : 8 * HALF;
+            const double inv_g = 1.0 / (double)G;  // x / G is the floor of (x + 1/2) / G, which f64 keeps apart from an integer
+            auto fold = [&](uint32_t r, uint32_t w0, float& M, float& L, f32x4& o, auto parts) {
+                constexpr uint32_t N = decltype(parts)::value, STEP = kWaves / N;
+                float mw[N], f[N];
+                f32x4 v[N];
+#pragma unroll
+                for (uint32_t i = 0; i < N; i++) {
+                    mw[i] = s_m[w0 + STEP * i][r];
+                    v[i] = *(const f32x4*)(s_kv + w0 * 2 * HALF + i * stride + r * 4 * D + (c ^ (r & (CH - 1))) * 16);
+                }
+                M = mw[0];
+#pragma unroll
+                for (uint32_t i = 1; i < N; i++) M = fmaxf(M, mw[i]);
+                L = 0.0f, o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t i = 0; i < N; i++) {
+                    f[i] = mw[i] == -INFINITY ? 0.0f : fast_exp2(mw[i] - M);  // (a wavefront that saw none of the row's positions: O is 0)
+                    L = __builtin_fmaf(s_l[w0 + STEP * i][r], f[i], L);
+                    o += v[i] * f[i];
+                }
+            };
+#pragma unroll 1
+            for (uint32_t rr = here(tid) / CH; rr < rows; rr += PER) {
+                float M, L;
+                f32x4 o;
+                if constexpr (narrow) fold(rr, 0, M, L, o, std::integral_constant<uint32_t, kWaves>{});
+                else fold(rr & 31, rr >> 5, M, L, o, std::integral_constant<uint32_t, 2>{});
+                const uint32_t packed = row0 + rr, token = (uint32_t)(((double)packed + 0.5) * inv_g), pos = before + token;
+                if (any_odd) {
+                    const PagedBatch& bt = p.a.batch;
+                    o = add_odd_values(p.a.v_pool + (uint64_t)kvh * bt.n_pages * bt.page_size * D,
+                                       bt.page_table + (uint64_t)wk.at.b * bt.max_pages, bt.page_size, bt.n_pages, D, kb,
+                                       min(end, pos + 1), c, o);
+                }
+                if (poison || pos >= bad_pos) M = 0.0f, L = NAN;
+                if (done || poison) {
+                    const uint64_t to = ((uint64_t)(start + token) * p.a.batch.n_q_heads + kvh * G + (packed - token * G)) * D + 4 * c;
+                    *(f32x4*)(p.a.out + to) = o * (1.0f / L);
+                } else {
+                    *(f32x4*)(p.part_o + ((uint64_t)slot * kRows + rr) * D + 4 * c) = o;
+                    if (c == 0) p.part_ml[(uint64_t)slot * kRows + rr] = float2{M, L};
+                }
             }
         }
         __syncthreads();  // LDS is free again
@@ -707,6 +891,9 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             w.at.j++;
             w.at.k = 0;
         }
+        };
+        if (uniform(wk.tile.rows) <= (uint32_t)kNarrow) piece(std::true_type{});
+        else piece(std::false_type{});
     }
 }
 
