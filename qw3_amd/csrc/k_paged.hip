@@ -175,13 +175,6 @@ struct AttnParams {
     MergeDesc* descs;  // [workgroups]
 };
 
-__device__ __forceinline__ f16x4 lds_read_tr16(const char* lds_ptr) {
-    typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 v4h;
-    typedef __attribute__((address_space(3))) v4h lds_v4h;
-    const v4h r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h*)(lds_ptr));
-    return __builtin_bit_cast(f16x4, r);
-}
-
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
     return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
 }
@@ -209,26 +202,30 @@ __device__ __forceinline__ void split2(float x0, float x1, f16x2& hi, f16x2& lo)
     hi = f16x2{(f16)x0, (f16)x1};
     lo = f16x2{(f16)(x0 - (float)hi[0]), (f16)(x1 - (float)hi[1])};
 }
-// The same of two weights (at least 0), both halves rounded towards 0 (one packed conversion each and
-// a mixed-precision fma per residual): 21 bits, 2^-22 too small in the mean.
+// The same of two weights in three instructions: a packed conversion that rounds towards 0, and each
+// residual x - hi as a mixed-precision fma that rounds its result to f16.
 __device__ __forceinline__ void split2_weights(float x0, float x1, f16x2& hi, f16x2& lo) {
     hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-    lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)hi[0], -1.0f, x0),
-                                                              __builtin_fmaf((float)hi[1], -1.0f, x1)));
+    const uint32_t h = __builtin_bit_cast(uint32_t, hi);
+    uint32_t l;
+    asm("v_fma_mixlo_f16 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]\n\t"
+        "v_fma_mixhi_f16 %0, %1, -1.0, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+        : "=&v"(l)
+        : "v"(h), "v"(x0), "v"(x1));
+    lo = __builtin_bit_cast(f16x2, l);
 }
 
 // The largest of a block's 16 scores on both lanes of a row. max3 as asm takes the products as they are
 // (compiled from fmaxf each operand is canonicalised first); the first maximum is compiled, so that it
 // waits for the products' result, and the others depend on it.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-    return r;
-}
 __device__ __forceinline__ float row_max(const f32x16& S) {
     float a = fmaxf(S[0], S[15]);
-#pragma unroll
-    for (int e = 1; e < 15; e += 2) a = max3(a, S[e], S[e + 1]);
+    asm("v_max3_f32 %0, %0, %1, %2\n\tv_max3_f32 %0, %0, %3, %4\n\tv_max3_f32 %0, %0, %5, %6\n\t"
+        "v_max3_f32 %0, %0, %7, %8\n\tv_max3_f32 %0, %0, %9, %10\n\tv_max3_f32 %0, %0, %11, %12\n\t"
+        "v_max3_f32 %0, %0, %13, %14"
+        : "+v"(a)
+        : "v"(S[1]), "v"(S[2]), "v"(S[3]), "v"(S[4]), "v"(S[5]), "v"(S[6]), "v"(S[7]), "v"(S[8]), "v"(S[9]), "v"(S[10]), "v"(S[11]),
+          "v"(S[12]), "v"(S[13]), "v"(S[14]));
     return swap32_op(a, OpMax{});
 }
 
@@ -339,25 +336,29 @@ struct Attn {
                 ((2 * (g16 & 1) + ((i16 & 3) >> 1)) ^ ds5idx::pb_swz(D, true, i16 >> 2)) * 16 + 8 * (i16 & 1);
         }
     };
-    // (a row's chunks are RB bytes aligned to RB, so xor in its low bits stays in the row)
-    __device__ __forceinline__ static f16x8 kread(const char* sk, const Lane& ln, int ks) {
-        return *(const f16x8*)(sk + (ln.k ^ (32 * ks)));
+    // Addresses: a block's base plus the lane's offset, then the swizzled chunk by xor (a block begins on a
+    // multiple of the row's RB bytes, so that xor in the low bits stays in the row).
+    __device__ __forceinline__ static f16x8 kread(uint32_t k, int ks) {
+        return *(const __attribute__((address_space(3))) f16x8*)(k ^ (32 * ks));
     }
     // positions 16 s + [0, 16): the transpose read gives lane i of 16 column i of 4 rows; element jj of the
     // operand is position 16 s + 8 (jj / 4) + 4 h + jj % 4, as the weights lie
-    __device__ __forceinline__ static f16x8 vread(const char* sv, const Lane& ln, int s, int dt) {
-        const char* at = sv + (ln.v ^ (64 * dt)) + 16 * s * RB;
-        const f16x4 a = lds_read_tr16(at), b = lds_read_tr16(at + 8 * RB);
+    __device__ __forceinline__ static f16x8 vread(uint32_t v, int s, int dt) {
+        typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 v4h;
+        typedef __attribute__((address_space(3))) v4h lds_v4h;
+        const uint32_t at = (v ^ (64 * dt)) + 16 * s * RB;
+        const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h*)at));
+        const f16x4 b = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h*)(at + 8 * RB)));
         return f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
     __device__ __forceinline__ void product(f32x16& S, const f16x8& k, int ks) const {
         S = mfma_32x32x16(k, qh[ks], S);
         if constexpr (!Q16) S = mfma_32x32x16(k, ql[ks], S);
     }
-    __device__ __forceinline__ void scores(f32x16& S, const char* sk, const Lane& ln) const {
+    __device__ __forceinline__ void scores(f32x16& S, uint32_t k) const {
         S = f32x16{};
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++) product(S, kread(sk, ln, ks), ks);
+        for (int ks = 0; ks < KS; ks++) product(S, kread(k, ks), ks);
     }
     __device__ __forceinline__ void mask_scores(f32x16& S, uint32_t key0, uint32_t end, uint32_t h) const {
         const int seen = (int)min(lim, end - 1) - (int)key0 - 4 * (int)h;
@@ -382,11 +383,11 @@ struct Attn {
 
     // One block by itself. scored(): called when the scores stand (K is read), landed(): before V is read.
     template <class Scored, class Landed>
-    __device__ __forceinline__ void block(const char* sk, const char* sv, uint32_t key0, uint32_t end, bool mask, Lane ln,
-                                          uint32_t h, Scored scored, Landed landed) {
+    __device__ __forceinline__ void block(uint32_t k, uint32_t v, uint32_t key0, uint32_t end, bool mask, uint32_t h,
+                                          Scored scored, Landed landed) {
         f32x16 S;
-        ln.k = here(ln.k), ln.v = here(ln.v);
-        scores(S, sk, ln);
+        k = here(k), v = here(v);
+        scores(S, k);
         scored();
         if (mask) mask_scores(S, key0, end, h);  // uniform
         rescale(row_max(S));
@@ -408,21 +409,20 @@ struct Attn {
         for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int dt = 0; dt < DT; dt++) {
-                const f16x8 v = vread(sv, ln, s, dt);
-                O[dt] = mfma_32x32x16(v, ph[s], O[dt]);
-                O[dt] = mfma_32x32x16(v, pl[s], O[dt]);
+                const f16x8 a = vread(v, s, dt);
+                O[dt] = mfma_32x32x16(a, ph[s], O[dt]);
+                O[dt] = mfma_32x32x16(a, pl[s], O[dt]);
             }
     }
 
-    // One block of a run of them: its scores S (largest mx) stand already; the products of the next block's
+    // One block of a run of them: its scores S (largest mx) stand already; the products of the next block's, Sn,
     // (K at sk; after the last block whatever lies there, its scores dropped) go beside the weights of S, the products with V beside the other half of the
     // weights and the next scores' maximum. load_k(), load_v(): later rows' loads, issued between products,
     // where the wait for the load path to take them costs nothing. LDS reads run kAhead operands ahead of their products. The
     // scheduling fences keep this order: a product occupies the matrix core for 32 cycles, in which the
     // wavefront issues the VALU work beside it.
     template <class LoadK, class LoadV>
-    __device__ __forceinline__ void step(f32x16& S, float& mx, const char* sk, const char* sv, Lane ln, LoadK load_k, LoadV load_v) {
-        ln.k = here(ln.k), ln.v = here(ln.v);
+    __device__ __forceinline__ void step(f32x16& S, f32x16& Sn, float& mx, uint32_t k, uint32_t v, LoadK load_k, LoadV load_v) {
         constexpr int kAhead = 3, NV = 2 * DT, E0 = 8 / KS, E1 = 8 / DT;
         rescale(mx);
         const float ref = reference();
@@ -439,24 +439,25 @@ struct Attn {
                 if (e % 8 == 7) asm volatile("" : "+v"(ph[e / 8]), "+v"(pl[e / 8]));  // here, not where they are used
             }
         };
-        f32x16 Sn = f32x16{};
+        k = here(k), v = here(v);
+        Sn = f32x16{};
 #pragma unroll
-        for (int n = 0; n < kAhead; n++) kop[n] = kread(sk, ln, n);
+        for (int n = 0; n < kAhead; n++) kop[n] = kread(k, n);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int n = 0; n < KS; n++) {
-            if (n + kAhead < KS) kop[n + kAhead] = kread(sk, ln, n + kAhead);
-            else vop[n + kAhead - KS] = vread(sv, ln, (n + kAhead - KS) / DT, (n + kAhead - KS) % DT);
+            if (n + kAhead < KS) kop[n + kAhead] = kread(k, n + kAhead);
+            else vop[n + kAhead - KS] = vread(v, (n + kAhead - KS) / DT, (n + kAhead - KS) % DT);
+#pragma unroll
+            for (int e = 0; e < E0; e++) weight(E0 * n + e);
             product(Sn, kop[n], n);
             if (n == 1) load_k();
             if (n == KS - 1) load_v();
-#pragma unroll
-            for (int e = 0; e < E0; e++) weight(E0 * n + e);
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int n = 0; n < NV; n++) {
-            if (n + kAhead < NV) vop[n + kAhead] = vread(sv, ln, (n + kAhead) / DT, (n + kAhead) % DT);
+            if (n + kAhead < NV) vop[n + kAhead] = vread(v, (n + kAhead) / DT, (n + kAhead) % DT);
             O[n % DT] = mfma_32x32x16(vop[n], ph[n / DT], O[n % DT]);
             O[n % DT] = mfma_32x32x16(vop[n], pl[n / DT], O[n % DT]);
             if (n < DT) {
@@ -467,7 +468,6 @@ struct Attn {
             __builtin_amdgcn_sched_barrier(0);
         }
         l += sum;
-        S = Sn;
     }
 
     // V rows of a block from position `end` on to zero (their weights are 0, what they hold may be
@@ -480,21 +480,37 @@ struct Attn {
         __builtin_amdgcn_wave_barrier();
     }
     __device__ __forceinline__ static bool clean(char* sv, uint32_t lane) {
+        constexpr int N = 4;  // chunks at a time: the wait for LDS counts once for each batch
         bool found = false;
+        static_assert(32 * RB / 16 % (64 * N) == 0, "whole batches");
 #pragma unroll 1
-        for (uint32_t c = here(lane); c < 32 * RB / 16; c += 64) {
-            u32x4 v = *(const u32x4*)(sv + 16 * c);
-            bool odd = false;
+        for (uint32_t c0 = here(lane); c0 < 32 * RB / 16; c0 += 64 * N) {
+            u32x4 v[N];
+            uint32_t odd = 0;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if ((v[i] & 0x7c00u) == 0x7c00u) v[i] &= 0xffff0000u, odd = true;
-                if ((v[i] & 0x7c000000u) == 0x7c000000u) v[i] &= 0xffffu, odd = true;
+            for (int j = 0; j < N; j++) v[j] = *(const u32x4*)(sv + 16 * (c0 + 64 * j));
+#pragma unroll
+            for (int j = 0; j < N; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {  // an exponent of all ones carries into bit 15 or 31 when one is added to it
+                    const uint32_t x = ((v[j][i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+                    odd |= x;
+                }
+            if (__ballot(odd != 0) != 0) {  // rare
+                found = true;
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if ((v[j][i] & 0x7c00u) == 0x7c00u) v[j][i] &= 0xffff0000u;
+                        if ((v[j][i] & 0x7c000000u) == 0x7c000000u) v[j][i] &= 0xffffu;
+                    }
+                    *(u32x4*)(sv + 16 * (c0 + 64 * j)) = v[j];
+                }
             }
-            if (odd) *(u32x4*)(sv + 16 * c) = v;
-            found = found || odd;
         }
         __builtin_amdgcn_wave_barrier();
-        return __ballot(found) != 0;
+        return found;
     }
 };
 
@@ -690,10 +706,10 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                     __syncthreads();
                     // element offset of the pool row of pos, a multiple of 8 (a page out of range: page 0, and the
                     // rows that attend it are NaN)
-                    auto row_of = [&](uint32_t pos) -> uint64_t {
-                        const uint32_t page = page_of(pos), pg = uniform(s_pages[page - page0]);
-                        return ((uint64_t)(pg < bt.n_pages ? pg : 0) * page_size + (pos - page * page_size)) * D;
+                    auto row_in = [&](uint32_t pos, uint32_t pg) -> uint64_t {
+                        return ((uint64_t)(pg < bt.n_pages ? pg : 0) * page_size + (pos - page_of(pos) * page_size)) * D;
                     };
+                    auto row_of = [&](uint32_t pos) { return row_in(pos, uniform(s_pages[page_of(pos) - page0])); };
                     if constexpr (narrow) {
                         // blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
                         // loaded once this one's scores stand, its V once this one's products do
@@ -722,7 +738,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                             const bool mask = masked(key0);
                             rows_at(next);
                             wait_loads<2 * NB>();  // K is here; V may not be
-                            t.block(sk, sv, key0, end, mask, ln, h,
+                            t.block(lds_addr(sk) + ln.k, lds_addr(sv) + ln.v, key0, end, mask, h,
                                     [&]() {
                                         if (next < to) load_k();
                                     },
@@ -744,47 +760,54 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                         constexpr uint32_t STAGE = 2 * 64 * RB;
                         const uint32_t steps = (to - from + 63) / 64, mine = 32 * (wave >> 2), last = (to - 1) / 8 * 8;
                         const uint32_t koff = t.koff ^ (wave & 1) * (RB / 2);  // the K rows' swizzle of rows 8 .. 15 of 16
-                        auto row_at = [&](uint32_t i) { return row_of(min(from + 64 * i + 8 * wave, last)); };
+                        auto pos_at = [&](uint32_t i) { return min(from + 64 * i + 8 * wave, last); };
+                        auto page_at = [&](uint32_t i) { return s_pages[page_of(pos_at(i)) - page0]; };
+                        auto row_at = [&](uint32_t i, uint32_t pg) { return row_in(pos_at(i), pg); };
                         auto lds_at = [&](uint32_t i) -> uint32_t { return lds_addr(s_kv) + (i & 3) * STAGE + 8 * wave * RB; };
-                        auto k_of = [&](uint32_t i) -> char* { return s_kv + (i & 3) * STAGE + mine * RB; };
+                        auto k_of = [&](uint32_t i) -> uint32_t { return lds_addr(s_kv) + (i & 3) * STAGE + mine * RB; };
                         // this wavefront's blocks: the first of the steps whose block holds a position its rows attend
                         const uint32_t upto = min(to, lim_hi + 1), first = from + mine;
                         const uint32_t blocks = 32 * rg < rows && upto > first ? (upto - first + 63) / 64 : 0;
                         for (uint32_t i = 0; i < 3; i++) {  // (steps past the last re-read its rows)
-                            const uint64_t r = row_at(i);
+                            const uint64_t r = row_at(i, uniform(page_at(i)));
                             A::template load_half<false>(lds_at(i), kpool + r, koff);
                             A::template load_half<true>(lds_at(i) + STAGE / 2, vpool + r, t.voff);
                         }
                         wait_loads<NB>();
                         __syncthreads();
-                        f32x16 S;
+                        f32x16 Sa, Sb;
                         float mx = -INFINITY;
                         if (blocks) {
-                            t.scores(S, k_of(0), ln);
-                            mx = row_max(S);
+                            t.scores(Sa, k_of(0) + ln.k);
+                            mx = row_max(Sa);
                         }
-#pragma unroll 1
-                        for (uint32_t i = 0; i < steps; i++) {
-                            const uint64_t r = row_at(i + 3);
+                        uint32_t page = page_at(3);
+                        auto run = [&](uint32_t i, f32x16& S, f32x16& Sn) {
+                            const uint64_t r = row_at(i + 3, uniform(page));
+                            page = page_at(i + 4);
                             auto load_k = [&]() { A::template load_half<false>(lds_at(i + 3), kpool + r, koff); };
                             auto load_v = [&]() { A::template load_half<true>(lds_at(i + 3) + STAGE / 2, vpool + r, t.voff); };
                             if (i < blocks) {
-                                const uint32_t key0 = first + 64 * i;
-                                char* const sv = k_of(i) + STAGE / 2;
+                                const uint32_t key0 = first + 64 * i, sv = k_of(i) + STAGE / 2;
                                 if (careful || masked(key0)) {
                                     if (masked(key0)) {
                                         t.mask_scores(S, key0, end, h);
                                         mx = row_max(S);
                                     }
-                                    clean(sv, key0);
+                                    clean(s_kv + (sv - lds_addr(s_kv)), key0);
                                 }
-                                t.step(S, mx, k_of(i + 1), sv, ln, load_k, load_v);
+                                t.step(S, Sn, mx, k_of(i + 1) + ln.k, sv + ln.v, load_k, load_v);
                             } else {
                                 load_k();
                                 load_v();
                             }
                             wait_loads<NB>();
                             __syncthreads();
+                        };
+#pragma unroll 1
+                        for (uint32_t i = 0; i < steps; i += 2) {  // (an odd count's last one works on nothing)
+                            run(i, Sa, Sb);
+                            run(i + 1, Sb, Sa);
                         }
                         wait_loads<0>();
                     }
