@@ -153,7 +153,7 @@ constexpr int kThreads = 512, kWaves = 8;
 constexpr int kRows = ds5idx::kPbRows, kNarrow = ds5idx::kPbNarrow;
 constexpr uint32_t kMaxSeqs = DS5_PAGED_MAX_SEQS;
 constexpr uint32_t kMaxGrid = 256;
-constexpr uint32_t kWindow = 1024;  // page table entries in LDS at a time
+constexpr uint32_t kWindow = 1024;  // groups of 16 positions whose place in the pool is in LDS at a time
 // Weights are exp2(score - reference): the reference starts 2^8 below the row's maximum and moves
 // when a weight would pass 2^15, so that in f16 hi + lo a weight keeps its 22 bits down to 2^-22
 // of the largest and counts down to 2^-33 of it.
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     __shared__ uint64_t s_scan[kWaves];
     __shared__ Walk s_walk;
     __shared__ uint32_t s_bad, s_odd, s_broken;
-    __shared__ uint32_t s_pages[kWindow];  // the page table's entries of a window of the piece
+    __shared__ uint32_t s_groups[kWindow];  // of a window of the piece: each 16 positions' group of rows in the pool
 
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = uniform(tid >> 6);
@@ -678,8 +678,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             const f16* const kpool = p.a.k_pool + head;
             const f16* const vpool = p.a.v_pool + head;
             const int32_t* const table = bt.page_table + (uint64_t)b * bt.max_pages;
-            const uint32_t page_size = bt.page_size, shift = p.page_shift;
-            auto page_of = [&](uint32_t pos) { return shift ? pos >> shift : pos / page_size; };
+            const uint32_t page_size = bt.page_size;
             bool careful = false;
             for (;;) {  // a second time, with infinities and NaN of V set aside, if the first left any in O
                 t.m = -INFINITY;
@@ -687,37 +686,33 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) t.O[dt] = f32x16{};
                 bool odd = false;
-                auto masked = [&](uint32_t key0) { return key0 + 31 > lim_lo || key0 + 32 > end; };
                 auto clean = [&](char* sv, uint32_t key0) {  // V rows that some row of the tile does not attend
                     if (key0 + 32 > end) A::zero_tail(sv, key0, end, lane);
                     if (careful || lim_hi > lim_lo) odd |= A::clean(sv, lane);
                 };
-                // the piece in windows of kWindow pages (most pieces are one)
+                // the piece in windows of kWindow groups of 16 positions (most pieces are one)
                 for (uint32_t from = poison ? end : kb, to; from < end; from = to) {
-                    const uint32_t page0 = uniform(page_of(from));
-                    const uint64_t window = ((uint64_t)page0 + kWindow) * page_size;
-                    to = window < end ? (uint32_t)window / 64 * 64 : end;
+                    to = end - from > 16 * kWindow ? from + 16 * kWindow : end;
+                    const uint32_t last = (to - from - 1) / 16;  // the window's last group; past it, it is read again
                     if (from > kb) __syncthreads();  // everyone is done with the window before
-                    for (uint32_t i = tid; i <= page_of(to - 1) - page0; i += kThreads) {
-                        const uint32_t pg = (uint32_t)table[page0 + i];
-                        s_pages[i] = pg;
-                        if (pg >= bt.n_pages) atomicMin(&s_bad, max(from, (page0 + i) * page_size));
+                    for (uint32_t i = tid; i <= last; i += kThreads) {
+                        const uint32_t pos = from + 16 * i, page = p.page_shift ? pos >> p.page_shift : pos / page_size;
+                        const uint32_t pg = (uint32_t)table[page];  // (a page out of range: page 0, and the rows that attend it are NaN)
+                        s_groups[i] = (pg < bt.n_pages ? pg : 0) * (page_size / 16) + (pos - page * page_size) / 16;
+                        if (pg >= bt.n_pages) atomicMin(&s_bad, pos);
                     }
                     __syncthreads();
-                    // element offset of the pool row of pos, a multiple of 8 (a page out of range: page 0, and the
-                    // rows that attend it are NaN)
-                    auto row_in = [&](uint32_t pos, uint32_t pg) -> uint64_t {
-                        return ((uint64_t)(pg < bt.n_pages ? pg : 0) * page_size + (pos - page_of(pos) * page_size)) * D;
-                    };
-                    auto row_of = [&](uint32_t pos) { return row_in(pos, uniform(s_pages[page_of(pos) - page0])); };
                     if constexpr (narrow) {
                         // blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
                         // loaded once this one's scores stand, its V once this one's products do
                         char* const sk = s_kv + wave * 2 * HALF;
                         char* const sv = sk + HALF;
-                        const uint32_t last = (to - 1) / 16 * 16;  // a group of positions past the end re-reads the last one
                         uint64_t r0, r1;
-                        auto rows_at = [&](uint32_t key0) { r0 = row_of(min(key0, last)), r1 = row_of(min(key0 + 16, last)); };
+                        auto rows_at = [&](uint32_t key0) {
+                            const uint32_t g = (key0 - from) / 16;
+                            r0 = (uint64_t)uniform(s_groups[min(g, last)]) * (16 * D);
+                            r1 = (uint64_t)uniform(s_groups[min(g + 1, last)]) * (16 * D);
+                        };
                         auto load_k = [&]() {
                             A::template load_group<false>(lds_addr(sk), kpool + r0, t.koff);
                             A::template load_group<false>(lds_addr(sk) + HALF / 2, kpool + r1, t.koff);
@@ -735,7 +730,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
 #pragma unroll 1
                         for (; key0 < to; key0 += 32 * kWaves) {
                             const uint32_t next = key0 + 32 * kWaves;
-                            const bool mask = masked(key0);
+                            const bool mask = key0 + 31 > lim_lo || key0 + 32 > end;
                             rows_at(next);
                             wait_loads<2 * NB>();  // K is here; V may not be
                             t.block(lds_addr(sk) + ln.k, lds_addr(sv) + ln.v, key0, end, mask, h,
@@ -758,48 +753,61 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                         // barrier; wavefronts 0 .. 3 take the first block of a step, 4 .. 7 the second. A step's K
                         // and V have landed one step before their block (its scores are formed a block ahead).
                         constexpr uint32_t STAGE = 2 * 64 * RB;
-                        const uint32_t steps = (to - from + 63) / 64, mine = 32 * (wave >> 2), last = (to - 1) / 8 * 8;
+                        const uint32_t steps = (to - from + 63) / 64, mine = 32 * (wave >> 2);
                         const uint32_t koff = t.koff ^ (wave & 1) * (RB / 2);  // the K rows' swizzle of rows 8 .. 15 of 16
-                        auto pos_at = [&](uint32_t i) { return min(from + 64 * i + 8 * wave, last); };
-                        auto page_at = [&](uint32_t i) { return s_pages[page_of(pos_at(i)) - page0]; };
-                        auto row_at = [&](uint32_t i, uint32_t pg) { return row_in(pos_at(i), pg); };
-                        auto lds_at = [&](uint32_t i) -> uint32_t { return lds_addr(s_kv) + (i & 3) * STAGE + 8 * wave * RB; };
-                        auto k_of = [&](uint32_t i) -> uint32_t { return lds_addr(s_kv) + (i & 3) * STAGE + mine * RB; };
-                        // this wavefront's blocks: the first of the steps whose block holds a position its rows attend
+                        const f16* const kw = kpool + (wave & 1) * 8 * D;
+                        const f16* const vw = vpool + (wave & 1) * 8 * D;
+                        const uint32_t lds0 = lds_addr(s_kv) + 8 * wave * RB;
+                        auto group_at = [&](uint32_t i) { return s_groups[min(4 * i + (wave >> 1), last)]; };
+                        auto load_k = [&](uint32_t i, uint32_t g) {
+                            A::template load_half<false>(lds0 + (i & 3) * STAGE, kw + (uint64_t)g * (16 * D), koff);
+                        };
+                        auto load_v = [&](uint32_t i, uint32_t g) {
+                            A::template load_half<true>(lds0 + (i & 3) * STAGE + STAGE / 2, vw + (uint64_t)g * (16 * D), t.voff);
+                        };
+                        const uint32_t k0 = lds_addr(s_kv) + mine * RB + ln.k, v0 = lds_addr(s_kv) + mine * RB + STAGE / 2 + ln.v;
+                        // this wavefront's blocks: the first of the steps whose block holds a position its rows attend;
+                        // those before `plain` need no mask
                         const uint32_t upto = min(to, lim_hi + 1), first = from + mine;
                         const uint32_t blocks = 32 * rg < rows && upto > first ? (upto - first + 63) / 64 : 0;
-                        for (uint32_t i = 0; i < 3; i++) {  // (steps past the last re-read its rows)
-                            const uint64_t r = row_at(i, uniform(page_at(i)));
-                            A::template load_half<false>(lds_at(i), kpool + r, koff);
-                            A::template load_half<true>(lds_at(i) + STAGE / 2, vpool + r, t.voff);
+                        const uint32_t whole = min(lim_lo + 1, end);  // positions below it all rows attend
+                        const uint32_t plain = careful || whole < first + 32 ? 0 : (whole - first - 32) / 64 + 1;
+                        {
+                            uint32_t g[3];
+#pragma unroll
+                            for (uint32_t i = 0; i < 3; i++) g[i] = group_at(i);
+#pragma unroll
+                            for (uint32_t i = 0; i < 3; i++) {  // (steps past the last re-read its rows)
+                                load_k(i, uniform(g[i]));
+                                load_v(i, uniform(g[i]));
+                            }
                         }
                         wait_loads<NB>();
                         __syncthreads();
                         f32x16 Sa, Sb;
                         float mx = -INFINITY;
                         if (blocks) {
-                            t.scores(Sa, k_of(0) + ln.k);
+                            t.scores(Sa, k0);
                             mx = row_max(Sa);
                         }
-                        uint32_t page = page_at(3);
+                        uint32_t ahead = group_at(3);
                         auto run = [&](uint32_t i, f32x16& S, f32x16& Sn) {
-                            const uint64_t r = row_at(i + 3, uniform(page));
-                            page = page_at(i + 4);
-                            auto load_k = [&]() { A::template load_half<false>(lds_at(i + 3), kpool + r, koff); };
-                            auto load_v = [&]() { A::template load_half<true>(lds_at(i + 3) + STAGE / 2, vpool + r, t.voff); };
+                            const uint32_t g = uniform(ahead);
+                            ahead = group_at(i + 4);
                             if (i < blocks) {
-                                const uint32_t key0 = first + 64 * i, sv = k_of(i) + STAGE / 2;
-                                if (careful || masked(key0)) {
-                                    if (masked(key0)) {
+                                if (__builtin_expect(i >= plain, 0)) {
+                                    const uint32_t key0 = first + 64 * i;
+                                    if (key0 + 31 > lim_lo || key0 + 32 > end) {
                                         t.mask_scores(S, key0, end, h);
                                         mx = row_max(S);
                                     }
-                                    clean(s_kv + (sv - lds_addr(s_kv)), key0);
+                                    clean(s_kv + (i & 3) * STAGE + STAGE / 2 + mine * RB, key0);
                                 }
-                                t.step(S, Sn, mx, k_of(i + 1) + ln.k, sv + ln.v, load_k, load_v);
+                                t.step(S, Sn, mx, k0 + ((i + 1) & 3) * STAGE, v0 + (i & 3) * STAGE, [&]() { load_k(i + 3, g); },
+                                       [&]() { load_v(i + 3, g); });
                             } else {
-                                load_k();
-                                load_v();
+                                load_k(i + 3, g);
+                                load_v(i + 3, g);
                             }
                             wait_loads<NB>();
                             __syncthreads();
