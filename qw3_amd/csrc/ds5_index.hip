@@ -167,12 +167,13 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
     const uint64_t total = per_head * n_kv_heads;
     if (!total) return 0;
     const uint32_t n_wg = whole ? grid : pb_workgroups(total, group, grid);
-    const uint64_t snap = pb_snap(total, n_wg, group);
+    const double share = 1.0 / (double)n_wg;
+    const uint64_t snap = pb_snap(total, share, group);
     uint64_t line = 0;
     auto cut = [&](uint32_t w) {
         if (w == n_wg) return PbCut{n_kv_heads, 0, 0, 0};
-        const uint64_t x = pb_cut_at(total, w, n_wg), y = x % per_head;
-        PbCut c{(uint32_t)(x / per_head), 0, 0, 0};
+        uint64_t y;
+        PbCut c{(uint32_t)pb_divide(pb_cut_at(total, w, n_wg, share), per_head, y), 0, 0, 0};
         uint64_t from = 0;
         for (;; c.b++) {
             const uint64_t work = n[c.b] ? pb_seq_work(seq(c.b), group) : 0;
@@ -196,7 +197,7 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
             if (count < max) {
                 const bool begins = at.k == 0 && end < t.kv;
                 const uint32_t row[10] = {w, at.kvh, at.b, ti, at.k, end, t.kv, t.row0, t.rows,
-                                          begins ? pb_last_cut(total, n_wg, tile_end - snap) : w};
+                                          begins ? pb_last_cut(total, n_wg, share, tile_end - snap) : w};
                 for (int i = 0; i < 10; i++) out[10 * count + i] = row[i];
             }
             count++;

@@ -207,7 +207,7 @@ DS5_HD uint32_t af_row_splits(uint32_t lim, uint32_t chunk) { return lim / chunk
 // were full) and kPbTileCost more. A cut inside a tile falls on a multiple of kPbUnit
 // positions of it, or on the tile's start or end where that is no further than `snap`.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 64;
+constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 256, kPbPiece = 128;
 
 struct PbSeq {
     uint32_t n, before;  // new tokens, and the tokens before them
@@ -238,12 +238,27 @@ DS5_HD uint64_t pb_before(PbSeq s, uint32_t group, uint32_t j) {
     const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
     return j / 2 * pair + (j % 2 ? pb_tile_work(s, group, nt - 1 - j / 2) : 0);
 }
+// x = q * d + r. (In f64, whose quotient is at most one off for x below 2^53: a 64-bit integer division
+// takes several times as long on the device.)
+DS5_HD uint64_t pb_divide(uint64_t x, uint64_t d, uint64_t& r) {
+    uint64_t q = (uint64_t)((double)x / (double)d);
+    int64_t left = (int64_t)(x - q * d);
+    if (left < 0) {
+        q--;
+        left += (int64_t)d;
+    } else if ((uint64_t)left >= d) {
+        q++;
+        left -= (int64_t)d;
+    }
+    r = (uint64_t)left;
+    return q;
+}
 // The cut at y of a sequence's work: tile j of its order (j may be one past the last), position k.
 DS5_HD void pb_locate(PbSeq s, uint32_t group, uint64_t y, uint64_t snap, bool whole, uint32_t& j, uint32_t& k) {
     const uint32_t nt = pb_tiles(s, group);
     const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
-    j = (uint32_t)(y / pair) * 2;
-    uint64_t off = y % pair;
+    uint64_t off;
+    j = (uint32_t)pb_divide(y, pair, off) * 2;
     const uint64_t heavy = pb_tile_work(s, group, pb_tile_at(j, nt));
     if (j + 1 < nt && off >= heavy) {
         j++;
@@ -264,18 +279,26 @@ DS5_HD void pb_locate(PbSeq s, uint32_t group, uint64_t y, uint64_t snap, bool w
     const uint32_t kv = pb_tile(s, group, tile).kv;
     k = umin((uint32_t)((double)kv * (double)off / (double)w), kv - 1) / kPbUnit * kPbUnit;
 }
-// The cut before workgroup w of n: x of a line of `work` (below 2^54, n below 2^9).
-DS5_HD uint64_t pb_cut_at(uint64_t work, uint32_t w, uint32_t n) { return work * w / n; }
-// The last workgroup whose cut is at most x (x below work).
-DS5_HD uint32_t pb_last_cut(uint64_t work, uint32_t n, uint64_t x) { return (uint32_t)(((x + 1) * n - 1) / work); }
-DS5_HD uint64_t pb_snap(uint64_t work, uint32_t n, uint32_t group) {
-    const uint64_t part = work / n / 16, least = (uint64_t)group * (kPbUnit / 2);
-    return part > least ? part : least;
+// The cut before workgroup w of n on a line of `work` (below 2^53): rounded, but never backwards as w
+// grows, and the same wherever it is worked out. part: 1.0 / n.
+DS5_HD uint64_t pb_cut_at(uint64_t work, uint32_t w, uint32_t n, double part) {
+    return w >= n ? work : (uint64_t)((double)work * ((double)w * part));
 }
-// The workgroups that share a line of work: 2 kPbUnit positions of a tile each at least.
+// The last workgroup whose cut is at most x (x below work).
+DS5_HD uint32_t pb_last_cut(uint64_t work, uint32_t n, double part, uint64_t x) {
+    uint32_t w = umin((uint32_t)((double)x / (double)work * (double)n), n - 1);
+    while (w > 0 && pb_cut_at(work, w, n, part) > x) w--;
+    while (w + 1 < n && pb_cut_at(work, w + 1, n, part) <= x) w++;
+    return w;
+}
+DS5_HD uint64_t pb_snap(uint64_t work, double part, uint32_t group) {
+    const uint64_t share = (uint64_t)((double)work * part * 0.0625), least = (uint64_t)group * (kPbUnit / 2);
+    return share > least ? share : least;
+}
+// The workgroups that share a line of work: kPbPiece positions of a tile each at least.
 DS5_HD uint32_t pb_workgroups(uint64_t work, uint32_t group, uint32_t grid) {
-    const uint64_t n = work / ((uint64_t)group * (2 * kPbUnit + kPbTileCost));
-    return n >= grid ? grid : n < 1 ? 1 : (uint32_t)n;
+    const double n = (double)work / ((double)group * kPbPiece);
+    return n >= (double)grid ? grid : n < 1.0 ? 1 : (uint32_t)n;
 }
 // Moves c on to the next tile that has rows; false where that is past the part that ends at `end`.
 // at_end: the part ends inside this tile, at position end.k. seq(b) gives sequence b.

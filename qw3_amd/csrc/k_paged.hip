@@ -258,41 +258,48 @@ struct Attn {
                          : "m0", "memory");
     }
 
-    // The lane's 8 elements of each k-step of its query row, at element `from` of q.
-    __device__ __forceinline__ void load_q(const AttnParams& p, uint64_t from) {
+    // The lane's 8 elements of each k-step of its query row, at element `from` of q: fetched, and made
+    // the products' operands once they are here.
+    struct Query {
+        f16x8 h[Q16 ? KS : 1];
+        float4 x0[Q16 ? 1 : KS], x1[Q16 ? 1 : KS];
+    };
+    __device__ __forceinline__ static void fetch_q(Query& q, const AttnParams& p, uint64_t from) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            if constexpr (Q16) {
+                q.h[ks] = *(const f16x8*)((const f16*)p.a.q + from + 16 * ks);
+            } else {
+                const float* src = (const float*)p.a.q + from + 16 * ks;
+                q.x0[ks] = *(const float4*)src;
+                q.x1[ks] = *(const float4*)(src + 4);
+            }
+        }
+    }
+    __device__ __forceinline__ void form_q(const Query& q, float scale) {
         // fac stays above 0 (a negative scale goes into the row's sign), so that the largest product is
         // the largest score and -inf stays -inf
-        const bool minus = p.a.scale < 0.0f;
-        const float scale_log2 = fmaxf(fabsf(p.a.scale * kLog2e), 1e-37f);
+        const bool minus = scale < 0.0f;
+        const float scale_log2 = fmaxf(fabsf(scale * kLog2e), 1e-37f);
         if constexpr (Q16) {
             fac = scale_log2;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                qh[ks] = *(const f16x8*)((const f16*)p.a.q + from + 16 * ks);
-                if (minus) qh[ks] = -qh[ks];
-            }
+            for (int ks = 0; ks < KS; ks++) qh[ks] = minus ? -q.h[ks] : q.h[ks];
         } else {
-            float4 q0[KS], q1[KS];
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const float* src = (const float*)p.a.q + from + 16 * ks;
-                q0[ks] = *(const float4*)src;
-                q1[ks] = *(const float4*)(src + 4);
-            }
             // the row times a power of two that brings its largest element to 2^13 .. 2^14: the
             // operands then hold 22 bits of it whatever its size
             float big = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
-                big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(q0[ks].x), fabsf(q0[ks].y)), fmaxf(fabsf(q0[ks].z), fabsf(q0[ks].w))),
-                                       fmaxf(fmaxf(fabsf(q1[ks].x), fabsf(q1[ks].y)), fmaxf(fabsf(q1[ks].z), fabsf(q1[ks].w)))));
+                big = fmaxf(big, fmaxf(fmaxf(fmaxf(fabsf(q.x0[ks].x), fabsf(q.x0[ks].y)), fmaxf(fabsf(q.x0[ks].z), fabsf(q.x0[ks].w))),
+                                       fmaxf(fmaxf(fabsf(q.x1[ks].x), fabsf(q.x1[ks].y)), fmaxf(fabsf(q.x1[ks].z), fabsf(q.x1[ks].w)))));
             big = swap32_op(big, OpMax{});
             const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 14 : 0;
             fac = fmaxf(ldexpf(scale_log2, e), 1e-37f);
             const float unit = minus ? -1.0f : 1.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                const float x[8] = {q0[ks].x, q0[ks].y, q0[ks].z, q0[ks].w, q1[ks].x, q1[ks].y, q1[ks].z, q1[ks].w};
+                const float x[8] = {q.x0[ks].x, q.x0[ks].y, q.x0[ks].z, q.x0[ks].w, q.x1[ks].x, q.x1[ks].y, q.x1[ks].z, q.x1[ks].w};
 #pragma unroll
                 for (int i = 0; i < 8; i += 2) {
                     f16x2 hi, lo;
@@ -532,7 +539,7 @@ __device__ __noinline__ f32x4 add_odd_values(const f16* vpool, const int32_t* ta
 // is read back by all, so that the loops over positions hold nothing of it in registers.
 struct Walk {
     ds5idx::PbCut at, stop;
-    uint64_t line, per_head, total;  // where the tile at `at` begins; one kv head's work, and all
+    uint64_t line, total;  // where the tile at `at` begins on the line; the line's length
     uint32_t wg, n_wg;
     uint32_t more, at_end;           // there is a piece; it is the last
     ds5idx::PbTile tile;
@@ -561,36 +568,36 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     {
         const PagedBatch& bt = p.a.batch;
         const uint32_t G = p.group;
-        uint64_t work[kMaxSeqs / kThreads];
+        constexpr uint32_t N = kMaxSeqs / kThreads;  // sequences a thread, consecutive ones
         uint64_t mine = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kMaxSeqs / kThreads; i++) {
-            const uint32_t b = tid * (kMaxSeqs / kThreads) + i;
-            work[i] = 0;
-            if (b < n_seqs) {
-                const int64_t s0 = bt.starts[b], s1 = bt.starts[b + 1], len = bt.seq_lens[b];
-                const int64_t c0 = max(s0, (int64_t)0), c1 = min(s1, (int64_t)bt.n_tokens);
-                const uint32_t n = c1 > c0 ? (uint32_t)(c1 - c0) : 0;
-                const bool ok = c0 == s0 && c1 == s1 && len >= s1 - s0 && len <= (int64_t)bt.max_seq_len;
-                s_start[b] = (uint32_t)c0;
-                s_n[b] = n;
-                s_before[b] = ok ? (uint32_t)(len - n) : kPoison;
-                if (n) work[i] = ds5idx::pb_seq_work(ds5idx::PbSeq{n, ok ? (uint32_t)(len - n) : 0u}, G);
-            }
-            mine += work[i];
+#pragma unroll 1
+        for (uint32_t b = tid * N; b < min(tid * N + N, n_seqs); b++) {
+            const int64_t s0 = bt.starts[b], s1 = bt.starts[b + 1], len = bt.seq_lens[b];
+            const int64_t c0 = max(s0, (int64_t)0), c1 = min(s1, (int64_t)bt.n_tokens);
+            const uint32_t n = c1 > c0 ? (uint32_t)(c1 - c0) : 0;
+            const bool ok = c0 == s0 && c1 == s1 && len >= s1 - s0 && len <= (int64_t)bt.max_seq_len;
+            s_start[b] = (uint32_t)c0;
+            s_n[b] = n;
+            s_before[b] = ok ? (uint32_t)(len - n) : kPoison;
+            mine += ds5idx::pb_seq_work(seq(b), G);
         }
         uint64_t upto = mine;  // inclusive over the wavefront
+        if (n_seqs > N) {
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint64_t y = __shfl_up(upto, o, 64);
-            if ((int)lane >= o) upto += y;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint64_t y = __shfl_up(upto, o, 64);
+                if ((int)lane >= o) upto += y;
+            }
         }
-        if (lane == 63) s_scan[wave] = upto;
+        if (lane == 63) s_scan[wave] = n_seqs > N ? upto : 0;
+        if (n_seqs <= N && tid == 0) s_scan[0] = mine;
         __syncthreads();
         uint64_t from = upto - mine, per_head = 0;
+#pragma unroll
         for (uint32_t w = 0; w < (uint32_t)kWaves; w++) {
-            from += w < wave ? s_scan[w] : 0;
-            per_head += s_scan[w];
+            const uint64_t x = s_scan[w];
+            from += w < wave ? x : 0;
+            per_head += x;
         }
         per_head = uniform64(per_head);
         const uint64_t total = per_head * bt.n_kv_heads;
@@ -601,30 +608,31 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         const uint32_t wg = n_wg == grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
         if (tid == 0 && p.descs) p.descs[wg].rows = 0;  // until it begins a tile that it does not end
         if (wg >= n_wg) return;
-        const uint64_t snap = ds5idx::pb_snap(total, n_wg, G);
-        const uint64_t x0 = ds5idx::pb_cut_at(total, wg, n_wg), x1 = ds5idx::pb_cut_at(total, wg + 1, n_wg);
-        const uint32_t h0 = (uint32_t)(x0 / per_head), h1 = (uint32_t)(x1 / per_head);
-        const uint64_t y0 = x0 - h0 * per_head, y1 = x1 - h1 * per_head;
+        const double share = 1.0 / (double)n_wg;
+        const uint64_t snap = ds5idx::pb_snap(total, share, G);
         if (tid == 0) {
-            s_walk.per_head = per_head, s_walk.total = total;
+            s_walk.total = total;
             s_walk.wg = wg, s_walk.n_wg = n_wg;
             s_walk.at_end = 0;
             if (wg + 1 == n_wg) s_walk.stop = ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0};
         }
-#pragma unroll
-        for (uint32_t i = 0; i < kMaxSeqs / kThreads; i++) {
-            const uint32_t b = tid * (kMaxSeqs / kThreads) + i;
-            uint32_t j, k;
-            if (y0 >= from && y0 - from < work[i]) {
-                ds5idx::pb_locate(seq(b), G, y0 - from, snap, p.whole, j, k);
-                s_walk.at = ds5idx::PbCut{h0, b, j, k};
-                s_walk.line = h0 * per_head + from + ds5idx::pb_before(seq(b), G, j);
+#pragma unroll 1
+        for (uint32_t c = 0; c < (wg + 1 < n_wg ? 2u : 1u); c++) {
+            uint64_t y, f = from;
+            const uint32_t h = (uint32_t)ds5idx::pb_divide(ds5idx::pb_cut_at(total, wg + c, n_wg, share), per_head, y);
+            if (y < from || y - from >= mine) continue;
+            for (uint32_t b = tid * N;; b++) {
+                const uint64_t work = ds5idx::pb_seq_work(seq(b), G);
+                if (y - f >= work) {
+                    f += work;
+                    continue;
+                }
+                uint32_t j, k;
+                ds5idx::pb_locate(seq(b), G, y - f, snap, p.whole, j, k);
+                (c ? s_walk.stop : s_walk.at) = ds5idx::PbCut{h, b, j, k};
+                if (c == 0) s_walk.line = h * per_head + f + ds5idx::pb_before(seq(b), G, j);
+                break;
             }
-            if (wg + 1 < n_wg && y1 >= from && y1 - from < work[i]) {
-                ds5idx::pb_locate(seq(b), G, y1 - from, snap, p.whole, j, k);
-                s_walk.stop = ds5idx::PbCut{h1, b, j, k};
-            }
-            from += work[i];
         }
     }
     __syncthreads();
@@ -672,13 +680,90 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             t.lim = before + row / G;
             const uint32_t lim_lo = uniform(before + (row0 + min(32 * rg, rows - 1)) / G);
             const uint32_t lim_hi = uniform(before + (row0 + min(32 * rg + 31, rows - 1)) / G);
-            t.load_q(p, ((uint64_t)(uniform(wk.start) + row / G) * bt.n_q_heads + kvh * G + row % G) * D + 8 * h);
+            typename A::Query query;
+            A::fetch_q(query, p, ((uint64_t)(uniform(wk.start) + row / G) * bt.n_q_heads + kvh * G + row % G) * D + 8 * h);
 
             const uint64_t head = (uint64_t)kvh * bt.n_pages * bt.page_size * D;
             const f16* const kpool = p.a.k_pool + head;
             const f16* const vpool = p.a.v_pool + head;
             const int32_t* const table = bt.page_table + (uint64_t)b * bt.max_pages;
             const uint32_t page_size = bt.page_size;
+            // The piece in windows of kWindow groups of 16 positions (most pieces are one): positions
+            // from .. to, `last` the last group; what is read past it is it again.
+            uint32_t from, to, last;
+            auto window = [&](uint32_t begin) {
+                from = begin;
+                to = end - from > 16 * kWindow ? from + 16 * kWindow : end;
+                last = (to - from - 1) / 16;
+#pragma unroll 1
+                for (uint32_t i = tid; i <= last; i += kThreads) {
+                    const uint32_t pos = from + 16 * i, page = p.page_shift ? pos >> p.page_shift : pos / page_size;
+                    const uint32_t pg = (uint32_t)table[page];  // (a page out of range: page 0, and the rows that attend it are NaN)
+                    s_groups[i] = (pg < bt.n_pages ? pg : 0) * (page_size / 16) + (pos - page * page_size) / 16;
+                    if (pg >= bt.n_pages) atomicMin(&s_bad, pos);
+                }
+                __syncthreads();
+            };
+            // narrow: blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
+            // loaded once this one's scores stand, its V once this one's products do
+            char* const sk = s_kv + wave * 2 * HALF;
+            char* const sv = sk + HALF;
+            uint64_t r0, r1;
+            auto rows_at = [&](uint32_t key0) {
+                const uint32_t g = (key0 - from) / 16;
+                r0 = (uint64_t)uniform(s_groups[min(g, last)]) * (16 * D);
+                r1 = (uint64_t)uniform(s_groups[min(g + 1, last)]) * (16 * D);
+            };
+            auto block_k = [&]() {
+                A::template load_group<false>(lds_addr(sk), kpool + r0, t.koff);
+                A::template load_group<false>(lds_addr(sk) + HALF / 2, kpool + r1, t.koff);
+            };
+            auto block_v = [&]() {
+                A::template load_group<true>(lds_addr(sv), vpool + r0, t.voff);
+                A::template load_group<true>(lds_addr(sv) + HALF / 2, vpool + r1, t.voff);
+            };
+            // wide: steps of 64 positions through a ring of four stages of K and V: wavefront w loads rows
+            // 8 w .. 8 w + 7, three steps ahead, into the stage that everyone left before the last barrier;
+            // wavefronts 0 .. 3 take the first block of a step, 4 .. 7 the second. A step's K and V have landed
+            // one step before their block (its scores are formed a block ahead).
+            constexpr uint32_t STAGE = 2 * 64 * RB;
+            const uint32_t mine = 32 * (wave >> 2);
+            const uint32_t koff = t.koff ^ (wave & 1) * (RB / 2);  // the K rows' swizzle of rows 8 .. 15 of 16
+            const f16* const kw = kpool + (wave & 1) * 8 * D;
+            const f16* const vw = vpool + (wave & 1) * 8 * D;
+            const uint32_t lds0 = lds_addr(s_kv) + 8 * wave * RB;
+            auto group_at = [&](uint32_t i) { return s_groups[min(4 * i + (wave >> 1), last)]; };
+            auto step_k = [&](uint32_t i, uint32_t g) {
+                A::template load_half<false>(lds0 + (i & 3) * STAGE, kw + (uint64_t)g * (16 * D), koff);
+            };
+            auto step_v = [&](uint32_t i, uint32_t g) {
+                A::template load_half<true>(lds0 + (i & 3) * STAGE + STAGE / 2, vw + (uint64_t)g * (16 * D), t.voff);
+            };
+            // a window's first loads
+            auto prime = [&]() {
+                if constexpr (narrow) {
+                    if (from + 32 * wave < to) {
+                        rows_at(from + 32 * wave);
+                        block_k();
+                        block_v();
+                    }
+                } else {
+                    uint32_t g[3];
+#pragma unroll
+                    for (uint32_t i = 0; i < 3; i++) g[i] = group_at(i);
+#pragma unroll
+                    for (uint32_t i = 0; i < 3; i++) {  // (steps past the last re-read its rows)
+                        step_k(i, uniform(g[i]));
+                        step_v(i, uniform(g[i]));
+                    }
+                }
+            };
+            const bool work = !poison && kb < end;
+            if (work) {
+                window(kb);
+                prime();
+            }
+            t.form_q(query, p.a.scale);  // while the first rows are on their way
             bool careful = false;
             for (;;) {  // a second time, with infinities and NaN of V set aside, if the first left any in O
                 t.m = -INFINITY;
@@ -690,52 +775,17 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                     if (key0 + 32 > end) A::zero_tail(sv, key0, end, lane);
                     if (careful || lim_hi > lim_lo) odd |= A::clean(sv, lane);
                 };
-                // the piece in windows of kWindow groups of 16 positions (most pieces are one)
-                for (uint32_t from = poison ? end : kb, to; from < end; from = to) {
-                    to = end - from > 16 * kWindow ? from + 16 * kWindow : end;
-                    const uint32_t last = (to - from - 1) / 16;  // the window's last group; past it, it is read again
-                    if (from > kb) __syncthreads();  // everyone is done with the window before
-                    for (uint32_t i = tid; i <= last; i += kThreads) {
-                        const uint32_t pos = from + 16 * i, page = p.page_shift ? pos >> p.page_shift : pos / page_size;
-                        const uint32_t pg = (uint32_t)table[page];  // (a page out of range: page 0, and the rows that attend it are NaN)
-                        s_groups[i] = (pg < bt.n_pages ? pg : 0) * (page_size / 16) + (pos - page * page_size) / 16;
-                        if (pg >= bt.n_pages) atomicMin(&s_bad, pos);
-                    }
-                    __syncthreads();
+                for (bool more = work; more;) {
                     if constexpr (narrow) {
-                        // blocks of 32 positions, one wavefront each, in an area of its own; the next block's K is
-                        // loaded once this one's scores stand, its V once this one's products do
-                        char* const sk = s_kv + wave * 2 * HALF;
-                        char* const sv = sk + HALF;
-                        uint64_t r0, r1;
-                        auto rows_at = [&](uint32_t key0) {
-                            const uint32_t g = (key0 - from) / 16;
-                            r0 = (uint64_t)uniform(s_groups[min(g, last)]) * (16 * D);
-                            r1 = (uint64_t)uniform(s_groups[min(g + 1, last)]) * (16 * D);
-                        };
-                        auto load_k = [&]() {
-                            A::template load_group<false>(lds_addr(sk), kpool + r0, t.koff);
-                            A::template load_group<false>(lds_addr(sk) + HALF / 2, kpool + r1, t.koff);
-                        };
-                        auto load_v = [&]() {
-                            A::template load_group<true>(lds_addr(sv), vpool + r0, t.voff);
-                            A::template load_group<true>(lds_addr(sv) + HALF / 2, vpool + r1, t.voff);
-                        };
-                        uint32_t key0 = from + 32 * wave;
-                        if (key0 < to) {
-                            rows_at(key0);
-                            load_k();
-                            load_v();
-                        }
 #pragma unroll 1
-                        for (; key0 < to; key0 += 32 * kWaves) {
+                        for (uint32_t key0 = from + 32 * wave; key0 < to; key0 += 32 * kWaves) {
                             const uint32_t next = key0 + 32 * kWaves;
                             const bool mask = key0 + 31 > lim_lo || key0 + 32 > end;
                             rows_at(next);
                             wait_loads<2 * NB>();  // K is here; V may not be
                             t.block(lds_addr(sk) + ln.k, lds_addr(sv) + ln.v, key0, end, mask, h,
                                     [&]() {
-                                        if (next < to) load_k();
+                                        if (next < to) block_k();
                                     },
                                     [&]() {
                                         if (next < to) wait_loads<2 * NB>();
@@ -744,27 +794,11 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                                     });
                             if (next < to) {
                                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                                load_v();
+                                block_v();
                             }
                         }
                     } else {
-                        // Steps of 64 positions through a ring of four stages of K and V: wavefront w loads rows
-                        // 8 w .. 8 w + 7, three steps ahead, into the stage that everyone left before the last
-                        // barrier; wavefronts 0 .. 3 take the first block of a step, 4 .. 7 the second. A step's K
-                        // and V have landed one step before their block (its scores are formed a block ahead).
-                        constexpr uint32_t STAGE = 2 * 64 * RB;
-                        const uint32_t steps = (to - from + 63) / 64, mine = 32 * (wave >> 2);
-                        const uint32_t koff = t.koff ^ (wave & 1) * (RB / 2);  // the K rows' swizzle of rows 8 .. 15 of 16
-                        const f16* const kw = kpool + (wave & 1) * 8 * D;
-                        const f16* const vw = vpool + (wave & 1) * 8 * D;
-                        const uint32_t lds0 = lds_addr(s_kv) + 8 * wave * RB;
-                        auto group_at = [&](uint32_t i) { return s_groups[min(4 * i + (wave >> 1), last)]; };
-                        auto load_k = [&](uint32_t i, uint32_t g) {
-                            A::template load_half<false>(lds0 + (i & 3) * STAGE, kw + (uint64_t)g * (16 * D), koff);
-                        };
-                        auto load_v = [&](uint32_t i, uint32_t g) {
-                            A::template load_half<true>(lds0 + (i & 3) * STAGE + STAGE / 2, vw + (uint64_t)g * (16 * D), t.voff);
-                        };
+                        const uint32_t steps = (to - from + 63) / 64;
                         const uint32_t k0 = lds_addr(s_kv) + mine * RB + ln.k, v0 = lds_addr(s_kv) + mine * RB + STAGE / 2 + ln.v;
                         // this wavefront's blocks: the first of the steps whose block holds a position its rows attend;
                         // those before `plain` need no mask
@@ -772,16 +806,6 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                         const uint32_t blocks = 32 * rg < rows && upto > first ? (upto - first + 63) / 64 : 0;
                         const uint32_t whole = min(lim_lo + 1, end);  // positions below it all rows attend
                         const uint32_t plain = careful || whole < first + 32 ? 0 : (whole - first - 32) / 64 + 1;
-                        {
-                            uint32_t g[3];
-#pragma unroll
-                            for (uint32_t i = 0; i < 3; i++) g[i] = group_at(i);
-#pragma unroll
-                            for (uint32_t i = 0; i < 3; i++) {  // (steps past the last re-read its rows)
-                                load_k(i, uniform(g[i]));
-                                load_v(i, uniform(g[i]));
-                            }
-                        }
                         wait_loads<NB>();
                         __syncthreads();
                         f32x16 Sa, Sb;
@@ -803,11 +827,11 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                                     }
                                     clean(s_kv + (i & 3) * STAGE + STAGE / 2 + mine * RB, key0);
                                 }
-                                t.step(S, Sn, mx, k0 + ((i + 1) & 3) * STAGE, v0 + (i & 3) * STAGE, [&]() { load_k(i + 3, g); },
-                                       [&]() { load_v(i + 3, g); });
+                                t.step(S, Sn, mx, k0 + ((i + 1) & 3) * STAGE, v0 + (i & 3) * STAGE, [&]() { step_k(i + 3, g); },
+                                       [&]() { step_v(i + 3, g); });
                             } else {
-                                load_k(i + 3, g);
-                                load_v(i + 3, g);
+                                step_k(i + 3, g);
+                                step_v(i + 3, g);
                             }
                             wait_loads<NB>();
                             __syncthreads();
@@ -818,6 +842,12 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                             run(i + 1, Sb, Sa);
                         }
                         wait_loads<0>();
+                    }
+                    more = to < end;
+                    if (more) {
+                        __syncthreads();  // everyone is done with the window
+                        window(to);
+                        prime();
                     }
                 }
                 if (odd && lane == 0) s_odd = 1;
@@ -830,6 +860,10 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                 __syncthreads();
                 if (careful || uniform(s_broken) == 0) break;
                 careful = true;
+                if (work) {
+                    window(kb);
+                    prime();
+                }
             }
         }
 
@@ -885,8 +919,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                     o += v[i] * f[i];
                 }
             };
-#pragma unroll 1
-            for (uint32_t rr = here(tid) / CH; rr < rows; rr += PER) {
+            auto finish = [&](uint32_t rr) {
                 float M, L;
                 f32x4 o;
                 if constexpr (narrow) fold(rr, 0, M, L, o, std::integral_constant<uint32_t, kWaves>{});
@@ -906,7 +939,13 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                     *(f32x4*)(p.part_o + ((uint64_t)slot * kRows + rr) * D + 4 * c) = o;
                     if (c == 0) p.part_ml[(uint64_t)slot * kRows + rr] = float2{M, L};
                 }
-            }
+            };
+            constexpr uint32_t U = narrow ? 1 : 4;  // rows at a time, for their reads from LDS to wait together
+#pragma unroll 1
+            for (uint32_t r = here(tid) / CH; r < rows; r += U * PER)
+#pragma unroll
+                for (uint32_t u = 0; u < U; u++)
+                    if (U == 1 || r + u * PER < rows) finish(r + u * PER);
         }
         __syncthreads();  // LDS is free again
         if (tid == 0) {
@@ -915,9 +954,11 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             const uint64_t tile_end =
                 w.line + ds5idx::pb_tile_work(sq, G, ds5idx::pb_tile_at(w.at.j, ds5idx::pb_tiles(sq, G)));
             // the last workgroup with a part of the tile: the last cut that is not within `snap` of its end
-            if (begins && !poison)
-                p.descs[wg] = MergeDesc{ds5idx::pb_last_cut(w.total, w.n_wg, tile_end - ds5idx::pb_snap(w.total, w.n_wg, G)), rows,
-                                        row0, kvh, start};
+            if (begins && !poison) {
+                const double share = 1.0 / (double)w.n_wg;
+                p.descs[wg] = MergeDesc{ds5idx::pb_last_cut(w.total, w.n_wg, share, tile_end - ds5idx::pb_snap(w.total, share, G)),
+                                        rows, row0, kvh, start};
+            }
             w.line = tile_end;
             w.at.j++;
             w.at.k = 0;
@@ -928,74 +969,106 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     }
 }
 
-// The parts of the tiles that several workgroups share, one tile per blockIdx.x: the head part of
-// workgroup w, then the parts of w + 1 .. last, folded in that order. 256 threads are D / 4 columns
-// and 1024 / D slots: with few parts a slot folds a row of its own, with many the slots share a
-// row's parts and join through LDS.
+// The parts of the tiles that several workgroups share: the head part of workgroup w, then the parts of
+// w + 1 .. last, folded in that order. 256 threads are D / 4 columns and 1024 / D slots: with few parts a
+// slot folds a row of its own, with many the slots share a row's parts and join through LDS. The
+// workgroups go along all tiles' rows (or groups of rows) evenly.
 template <int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(AttnParams p) {
-    constexpr int CH = D / 4, SL = 256 / CH;
+__global__ __launch_bounds__(kMaxGrid) void paged_merge_kernel(AttnParams p, uint32_t n_descs) {
+    constexpr uint32_t CH = D / 4, SL = kMaxGrid / CH;
+    __shared__ uint32_t s_upto[kMaxGrid];  // items of the tiles up to and with this one
+    __shared__ uint32_t s_wave[kMaxGrid / 64], s_item;
     __shared__ f32x4 s_o[SL][CH];
     __shared__ float2 s_ml[SL];
-    const MergeDesc d = p.descs[blockIdx.x];
-    if (d.rows == 0) return;
-    const uint32_t w = blockIdx.x, n = d.last - w + 1, G = p.group;
-    const uint32_t c = threadIdx.x % CH, sl = threadIdx.x / CH;
-    auto slot_of = [&](uint32_t i) -> uint64_t { return i == 0 ? 2 * w + 1 : 2 * (w + i); };
-    // parts first, first + step, ... of a row
-    auto fold = [&](uint32_t row, uint32_t first, uint32_t step, float& M, float& L, f32x4& o) {
-        constexpr int U = 4;
-        M = -INFINITY, L = 0.0f, o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (uint32_t i0 = first; i0 < n; i0 += U * step) {
-            float2 ml[U];
-            f32x4 v[U];
+    const uint32_t tid = threadIdx.x, lane = tid & 63, G = p.group;
+    auto together = [&](uint32_t parts) { return parts <= SL; };  // SL rows at once
+    MergeDesc mine{};
+    if (tid < n_descs) mine = p.descs[tid];
+    const uint32_t items = mine.rows == 0 ? 0 : together(mine.last - tid + 1) ? (mine.rows + SL - 1) / SL : mine.rows;
+    uint32_t upto = items;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const uint64_t s = slot_of(min(i0 + u * step, n - 1)) * kRows + row;
-                ml[u] = p.part_ml[s];
-                v[u] = *(const f32x4*)(p.part_o + s * D + 4 * c);
-            }
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t y = __shfl_up(upto, o, 64);
+        if ((int)lane >= o) upto += y;
+    }
+    if (lane == 63) s_wave[tid >> 6] = upto;
+    __syncthreads();
+    uint32_t total = 0;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (i0 + u * step >= n || ml[u].x == -INFINITY) continue;
-                const float m = fmaxf(M, ml[u].x), fa = M == -INFINITY ? 0.0f : fast_exp2(M - m), fb = fast_exp2(ml[u].x - m);
-                L = L * fa + ml[u].y * fb;
-                o = o * fa + v[u] * fb;
+    for (uint32_t w = 0; w < kMaxGrid / 64; w++) {
+        if (w < tid >> 6) upto += s_wave[w];
+        total += s_wave[w];
+    }
+    s_upto[tid] = upto;
+    __syncthreads();
+    const uint32_t c = tid % CH, sl = tid / CH;
+    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
+        if (item < upto && item >= upto - items) s_item = tid;  // one thread's
+        __syncthreads();
+        const uint32_t w = uniform(s_item);
+        const MergeDesc d = p.descs[w];
+        const uint32_t n = d.last - w + 1, at = item - (w ? s_upto[w - 1] : 0);
+        // parts first, first + step, ... of a row
+        auto fold = [&](uint32_t row, uint32_t first, uint32_t step, float& M, float& L, f32x4& o) {
+            constexpr int U = 8;
+            M = -INFINITY, L = 0.0f, o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t i0 = first; i0 < n; i0 += U * step) {
+                float2 ml[U];
+                f32x4 v[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const uint32_t i = min(i0 + u * step, n - 1);
+                    const uint64_t s = (uint64_t)(i == 0 ? 2 * w + 1 : 2 * (w + i)) * kRows + row;
+                    ml[u] = p.part_ml[s];
+                    v[u] = *(const f32x4*)(p.part_o + s * D + 4 * c);
+                }
+                float m = M;
+#pragma unroll
+                for (int u = 0; u < U; u++) m = i0 + u * step < n ? fmaxf(m, ml[u].x) : m;
+                const float f0 = M == -INFINITY ? 0.0f : fast_exp2(M - m);
+                L *= f0, o *= f0;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (i0 + u * step < n && ml[u].x != -INFINITY) {  // (a part of none of the row's positions holds nothing)
+                        const float f = fast_exp2(ml[u].x - m);
+                        L = __builtin_fmaf(ml[u].y, f, L);
+                        o += v[u] * f;
+                    }
                 M = m;
             }
-        }
-    };
-    auto write = [&](uint32_t row, f32x4 o, float L) {
-        const uint32_t packed = d.row0 + row;
-        *(f32x4*)(p.a.out + ((uint64_t)(d.token0 + packed / G) * p.a.batch.n_q_heads + d.kvh * G + packed % G) * D + 4 * c) = o / L;
-    };
-    float M, L;
-    f32x4 o;
-    if (n <= 4) {
-        for (uint32_t row = blockIdx.y * SL + sl; row < d.rows; row += gridDim.y * SL) {
-            fold(row, 0, 1, M, L, o);
-            write(row, o, L);
-        }
-        return;
-    }
-    for (uint32_t row = blockIdx.y; row < d.rows; row += gridDim.y) {
-        fold(row, sl, SL, M, L, o);
-        __syncthreads();
-        s_o[sl][c] = o;
-        if (c == 0) s_ml[sl] = float2{M, L};
-        __syncthreads();
-        if (sl == 0) {
-            float mm = -INFINITY, ll = 0.0f;
-            for (int i = 0; i < SL; i++) mm = fmaxf(mm, s_ml[i].x);
-            f32x4 oo = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int i = 0; i < SL; i++) {
-                if (s_ml[i].x == -INFINITY) continue;
-                const float f = fast_exp2(s_ml[i].x - mm);
-                ll += s_ml[i].y * f;
-                oo += s_o[i][c] * f;
+        };
+        auto write = [&](uint32_t row, f32x4 o, float L) {
+            const uint32_t packed = d.row0 + row;
+            *(f32x4*)(p.a.out + ((uint64_t)(d.token0 + packed / G) * p.a.batch.n_q_heads + d.kvh * G + packed % G) * D + 4 * c) =
+                o * (1.0f / L);
+        };
+        float M, L;
+        f32x4 o;
+        if (together(n)) {
+            const uint32_t row = at * SL + sl;
+            if (row < d.rows) {
+                fold(row, 0, 1, M, L, o);
+                write(row, o, L);
             }
-            write(row, oo, ll);
+        } else {
+            fold(at, sl, SL, M, L, o);
+            s_o[sl][c] = o;
+            if (c == 0) s_ml[sl] = float2{M, L};
+            __syncthreads();
+            if (sl == 0) {
+                float mm = -INFINITY, ll = 0.0f;
+                for (uint32_t i = 0; i < SL; i++) mm = fmaxf(mm, s_ml[i].x);
+                f32x4 oo = {0.0f, 0.0f, 0.0f, 0.0f};
+                for (uint32_t i = 0; i < SL; i++) {
+                    if (s_ml[i].x == -INFINITY) continue;
+                    const float f = fast_exp2(s_ml[i].x - mm);
+                    ll += s_ml[i].y * f;
+                    oo += s_o[i][c] * f;
+                }
+                write(at, oo, ll);
+            }
         }
+        __syncthreads();  // s_item, s_o and s_ml are free again
     }
 }
 
@@ -1021,13 +1094,14 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     p.group = b.n_q_heads / b.n_kv_heads;
     p.page_shift = (b.page_size & (b.page_size - 1)) == 0 ? (uint32_t)__builtin_ctz(b.page_size) : 0;
     const uint64_t rows = (uint64_t)b.n_tokens * p.group, tiles = rows / kRows + std::min<uint64_t>(b.n_seqs, b.n_tokens);
-    // the work that the plan counts, at most: below 2^54
-    if ((double)b.n_kv_heads * tiles * ((double)p.group * ((double)b.max_seq_len + kRows) + rows + kRows) >= 18014398509481984.0)
+    // the work that the plan counts, at most: below 2^53
+    if ((double)b.n_kv_heads * tiles * ((double)p.group * ((double)b.max_seq_len + ds5idx::kPbTileCost) + rows + kRows) >= 9007199254740992.0)
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "paged_attention: batch too large");
     // Up to 256 positions a workgroup's eight wavefronts take a tile in one go: none is cut then,
     // and nothing merged. (Nor without the context's memory for parts.)
     p.whole = !ctx->split_buf || b.max_seq_len <= 256;
-    const uint64_t most = b.n_kv_heads * tiles * (p.whole ? 1 : ((uint64_t)b.max_seq_len + 2 * ds5idx::kPbUnit - 1) / (2 * ds5idx::kPbUnit));
+    const uint64_t most =
+        b.n_kv_heads * tiles * (p.whole ? 1 : ((uint64_t)b.max_seq_len + ds5idx::kPbTileCost) / ds5idx::kPbPiece + 1);
     const uint32_t cus = std::min(kMaxGrid, ctx->cu_count > 0 ? (uint32_t)ctx->cu_count : kMaxGrid);
     const dim3 grid((uint32_t)std::min<uint64_t>(most, cus)), block(kThreads);
     if (!p.whole) {
@@ -1047,9 +1121,10 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     }
     if (int rc = ds5_after_launch(ctx, name)) return rc;
     if (p.whole || grid.x == 1) return DS5_OK;  // one workgroup cuts nothing
-    const dim3 merge(grid.x, (uint32_t)std::min<uint64_t>(rows, 16));
+    // an item is a row at least, and there are n_q_heads of a token
+    const dim3 merge((uint32_t)std::min<uint64_t>((uint64_t)b.n_tokens * b.n_q_heads, 4 * kMaxGrid));
     name = "paged_merge_kernel";
-    if (b.head_dim == 128) DS5_TIMED_LAUNCH(ctx, name, paged_merge_kernel<128>, merge, dim3(256), 0, ctx->stream, p);
-    else DS5_TIMED_LAUNCH(ctx, name, paged_merge_kernel<64>, merge, dim3(256), 0, ctx->stream, p);
+    if (b.head_dim == 128) DS5_TIMED_LAUNCH(ctx, name, paged_merge_kernel<128>, merge, dim3(kMaxGrid), 0, ctx->stream, p, grid.x);
+    else DS5_TIMED_LAUNCH(ctx, name, paged_merge_kernel<64>, merge, dim3(kMaxGrid), 0, ctx->stream, p, grid.x);
     return ds5_after_launch(ctx, name);
 }
