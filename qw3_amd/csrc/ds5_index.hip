@@ -166,7 +166,7 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
     for (uint32_t b = 0; b < n_seqs; b++) per_head += n[b] ? pb_seq_work(seq(b), group) : 0;
     const uint64_t total = per_head * n_kv_heads;
     if (!total) return 0;
-    const uint32_t n_wg = whole ? grid : pb_workgroups(total, group, grid);
+    const uint32_t n_wg = whole ? grid : pb_workgroups(total, group, n_kv_heads, grid);
     const double share = 1.0 / (double)n_wg;
     const uint64_t snap = pb_snap(total, share, group);
     uint64_t line = 0;

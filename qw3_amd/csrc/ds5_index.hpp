@@ -204,10 +204,12 @@ DS5_HD uint32_t af_row_splits(uint32_t lim, uint32_t chunk) { return lim / chunk
 // tile in the order last, first, last but one, second, ... (a pair of them costs the same for
 // every pair), its positions. Workgroup w of n takes the part from w / n to (w + 1) / n of it.
 // Work is counted in positions * group, a tile's being its positions (taken as if every tile
-// were full) and kPbTileCost more. A cut inside a tile falls on a multiple of kPbUnit
+// were full) and kPbTileCost more, twice for the tiles of sequences of more than kPbNarrow rows
+// (64 positions of a tile of 128 rows take 1.5 us, of one of 32 rows 0.7 where the caches'
+// rows arrive in time; beginning and ending a tile 8 and 5). A cut inside a tile falls on a multiple of kPbUnit
 // positions of it, or on the tile's start or end where that is no further than `snap`.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 256, kPbPiece = 128;
+constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 512, kPbPiece = 192;
 
 struct PbSeq {
     uint32_t n, before;  // new tokens, and the tokens before them
@@ -220,12 +222,13 @@ struct PbCut {
 };
 
 DS5_HD uint32_t pb_tiles(PbSeq s, uint32_t group) { return (s.n * group + kPbRows - 1) / kPbRows; }
+DS5_HD uint32_t pb_weight(PbSeq s, uint32_t group) { return s.n * group > kPbNarrow ? 2 : 1; }
 DS5_HD uint64_t pb_tile_work(PbSeq s, uint32_t group, uint32_t tile) {
-    return (uint64_t)group * ((uint64_t)s.before + kPbTileCost) + (uint64_t)kPbRows * (tile + 1);
+    return pb_weight(s, group) * ((uint64_t)group * ((uint64_t)s.before + kPbTileCost) + (uint64_t)kPbRows * (tile + 1));
 }
 DS5_HD uint64_t pb_seq_work(PbSeq s, uint32_t group) {
     const uint64_t nt = pb_tiles(s, group);
-    return nt * group * ((uint64_t)s.before + kPbTileCost) + kPbRows / 2 * nt * (nt + 1);
+    return pb_weight(s, group) * (nt * group * ((uint64_t)s.before + kPbTileCost) + kPbRows / 2 * nt * (nt + 1));
 }
 DS5_HD uint32_t pb_tile_at(uint32_t j, uint32_t nt) { return j % 2 ? j / 2 : nt - 1 - j / 2; }
 DS5_HD PbTile pb_tile(PbSeq s, uint32_t group, uint32_t tile) {
@@ -295,10 +298,12 @@ DS5_HD uint64_t pb_snap(uint64_t work, double part, uint32_t group) {
     const uint64_t share = (uint64_t)((double)work * part * 0.0625), least = (uint64_t)group * (kPbUnit / 2);
     return share > least ? share : least;
 }
-// The workgroups that share a line of work: kPbPiece positions of a tile each at least.
-DS5_HD uint32_t pb_workgroups(uint64_t work, uint32_t group, uint32_t grid) {
+// The workgroups that share a line of work: kPbPiece positions of a tile each at least, and the same number
+// for each kv head where there are enough, so that no workgroup ends one head's tile to begin another's.
+DS5_HD uint32_t pb_workgroups(uint64_t work, uint32_t group, uint32_t heads, uint32_t grid) {
     const double n = (double)work / ((double)group * kPbPiece);
-    return n >= (double)grid ? grid : n < 1.0 ? 1 : (uint32_t)n;
+    const uint32_t all = n >= (double)grid ? grid : n < 1.0 ? 1 : (uint32_t)n;
+    return all > heads ? all / heads * heads : all;
 }
 // Moves c on to the next tile that has rows; false where that is past the part that ends at `end`.
 // at_end: the part ends inside this tile, at position end.k. seq(b) gives sequence b.

@@ -234,6 +234,7 @@ struct Attn {
     static constexpr int KS = D / 16, DT = D / 32, RB = 2 * D;
     static constexpr int NB = 16 * RB / 1024;      // direct-to-LDS loads of a group of 16 rows
     static constexpr int HALF = 32 * RB;           // bytes of 32 rows
+    static_assert(kRows * D * 4 <= kWaves * HALF, "a tile's query rows fit half of the area");
     static constexpr int AREA = kWaves * 2 * HALF; // K and V of a block for each wavefront, or four stages of two blocks
     static constexpr int CH = D / 4;               // float4 of an O row
 
@@ -273,6 +274,34 @@ struct Attn {
                 const float* src = (const float*)p.a.q + from + 16 * ks;
                 q.x0[ks] = *(const float4*)src;
                 q.x1[ks] = *(const float4*)(src + 4);
+            }
+        }
+    }
+    // The rows of a wide tile through LDS, where their loads run along rows (in the operands' layout each load
+    // instruction touches 64 cache lines: 3.7 us of a tile's 128 rows of f32): wavefront w loads rows 16 w ..
+    // 16 w + 15, 16-byte chunk c of row r into the row's slot c ^ qswz(r).
+    static constexpr int QB = D * (Q16 ? 2 : 4), QC = QB / 16;
+    __device__ __forceinline__ static uint32_t qswz(uint32_t r) { return QC == 8 ? (r >> 1) & 7 : r & (QC - 1); }
+    template <class RowOf>
+    __device__ __forceinline__ static void stage_q(uint32_t lds, const void* q, uint32_t wave, uint32_t lane, RowOf row_of) {
+#pragma unroll
+        for (int j = 0; j < 16 * QB / 1024; j++) {
+            const uint32_t at = 1024 * j + 16 * lane, r = 16 * wave + at / QB, slot = at % QB / 16;
+            const char* src = (const char*)q + row_of(r) * QB + (slot ^ qswz(r)) * 16;
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
+                         "s"(uniform(lds + 16 * wave * QB + 1024 * j))
+                         : "m0", "memory");
+        }
+    }
+    __device__ __forceinline__ static void staged_q(Query& q, const char* sq, uint32_t r, uint32_t h) {
+        const char* row = sq + r * QB;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            if constexpr (Q16) {
+                q.h[ks] = *(const f16x8*)(row + ((2 * ks + h) ^ qswz(r)) * 16);
+            } else {
+                q.x0[ks] = *(const float4*)(row + ((4 * ks + 2 * h) ^ qswz(r)) * 16);
+                q.x1[ks] = *(const float4*)(row + ((4 * ks + 2 * h + 1) ^ qswz(r)) * 16);
             }
         }
     }
@@ -602,10 +631,10 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         per_head = uniform64(per_head);
         const uint64_t total = per_head * bt.n_kv_heads;
         const uint32_t grid = gridDim.x;
-        const uint32_t n_wg = total == 0 ? 0 : p.whole ? grid : ds5idx::pb_workgroups(total, G, grid);
+        const uint32_t n_wg = total == 0 ? 0 : p.whole ? grid : ds5idx::pb_workgroups(total, G, bt.n_kv_heads, grid);
         // A full grid's consecutive parts go to one XCD (workgroup i runs on XCD i % 8), so that a
         // sequence's K and V come into few L2s.
-        const uint32_t wg = n_wg == grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
+        const uint32_t wg = n_wg + bt.n_kv_heads > grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
         if (tid == 0 && p.descs) p.descs[wg].rows = 0;  // until it begins a tile that it does not end
         if (wg >= n_wg) return;
         const double share = 1.0 / (double)n_wg;
@@ -681,7 +710,16 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             const uint32_t lim_lo = uniform(before + (row0 + min(32 * rg, rows - 1)) / G);
             const uint32_t lim_hi = uniform(before + (row0 + min(32 * rg + 31, rows - 1)) / G);
             typename A::Query query;
-            A::fetch_q(query, p, ((uint64_t)(uniform(wk.start) + row / G) * bt.n_q_heads + kvh * G + row % G) * D + 8 * h);
+            const uint32_t start = uniform(wk.start);
+            if constexpr (narrow)
+                A::fetch_q(query, p, ((uint64_t)(start + row / G) * bt.n_q_heads + kvh * G + row % G) * D + 8 * h);
+            else {
+                const double inv_g = 1.0 / (double)G;  // x / G is the floor of (x + 1/2) / G, which f64 keeps apart from an integer
+                A::stage_q(lds_addr(s_kv) + A::AREA / 2, p.a.q, wave, lane, [&](uint32_t r) -> uint64_t {
+                    const uint32_t packed = row0 + min(r, rows - 1), token = (uint32_t)(((double)packed + 0.5) * inv_g);
+                    return (uint64_t)(start + token) * bt.n_q_heads + kvh * G + (packed - token * G);
+                });
+            }
 
             const uint64_t head = (uint64_t)kvh * bt.n_pages * bt.page_size * D;
             const f16* const kpool = p.a.k_pool + head;
@@ -759,9 +797,26 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                 }
             };
             const bool work = !poison && kb < end;
-            if (work) {
-                window(kb);
-                prime();
+            if (work) window(kb);
+            if constexpr (narrow) {
+                if (work) prime();
+            } else {
+                if (work) {
+                    for (uint32_t i = 0; i < 2; i++) {
+                        const uint32_t g = uniform(group_at(i));
+                        step_k(i, g);
+                        step_v(i, g);
+                    }
+                }
+                wait_loads<0>();
+                __syncthreads();
+                A::staged_q(query, s_kv + A::AREA / 2, 32 * rg + r32, h);
+                __syncthreads();  // the query rows' area is the ring's other half
+                if (work) {
+                    const uint32_t g = uniform(group_at(2));
+                    step_k(2, g);
+                    step_v(2, g);
+                }
             }
             t.form_q(query, p.a.scale);  // while the first rows are on their way
             bool careful = false;
@@ -1095,13 +1150,13 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     p.page_shift = (b.page_size & (b.page_size - 1)) == 0 ? (uint32_t)__builtin_ctz(b.page_size) : 0;
     const uint64_t rows = (uint64_t)b.n_tokens * p.group, tiles = rows / kRows + std::min<uint64_t>(b.n_seqs, b.n_tokens);
     // the work that the plan counts, at most: below 2^53
-    if ((double)b.n_kv_heads * tiles * ((double)p.group * ((double)b.max_seq_len + ds5idx::kPbTileCost) + rows + kRows) >= 9007199254740992.0)
+    if (2.0 * b.n_kv_heads * tiles * ((double)p.group * ((double)b.max_seq_len + ds5idx::kPbTileCost) + rows + kRows) >= 9007199254740992.0)
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "paged_attention: batch too large");
     // Up to 256 positions a workgroup's eight wavefronts take a tile in one go: none is cut then,
     // and nothing merged. (Nor without the context's memory for parts.)
     p.whole = !ctx->split_buf || b.max_seq_len <= 256;
     const uint64_t most =
-        b.n_kv_heads * tiles * (p.whole ? 1 : ((uint64_t)b.max_seq_len + ds5idx::kPbTileCost) / ds5idx::kPbPiece + 1);
+        b.n_kv_heads * tiles * (p.whole ? 1 : 2 * ((uint64_t)b.max_seq_len + ds5idx::kPbTileCost) / ds5idx::kPbPiece + 1);
     const uint32_t cus = std::min(kMaxGrid, ctx->cu_count > 0 ? (uint32_t)ctx->cu_count : kMaxGrid);
     const dim3 grid((uint32_t)std::min<uint64_t>(most, cus)), block(kThreads);
     if (!p.whole) {
