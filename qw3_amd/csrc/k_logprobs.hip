@@ -14,11 +14,11 @@
 // segments' states. Memory bound: the logits are read once.
 //
 // Selection by unique 64-bit keys (the logit in an order-preserving form above the complement of
-// its index, so that equal logits fall to the lower index): every thread's largest key; the
-// top_n-th largest of those is a bound that at least top_n elements reach, and only the elements
-// of the top_n threads whose largest reaches it can (at most PER * top_n; a few more than top_n
-// as a rule). They are gathered in LDS and ordered by counting, for each, those above it. The
-// join does the same with each segment's sorted keys in place of a thread's elements.
+// its index, so that equal logits fall to the lower index): a bound that top_n to 1.5 top_n of the
+// threads' largest keys reach is one that top_n elements reach, and only those threads' elements
+// can (at most 1.5 PER top_n; a few more than top_n as a rule). They are gathered in LDS and
+// ordered by counting, for each, those above it. The join does the same with each segment's
+// sorted keys in place of a thread's elements.
 #include "ds5_common.hpp"
 
 namespace {
@@ -51,56 +51,73 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
 
 __device__ __forceinline__ uint64_t kmax(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// The n largest of the keys that the threads' lists hold, in descending order into out[0, n) (0
-// where there are fewer). own: the thread's largest key (0: none); each(f) calls f for the keys
-// of its list that may reach `bound`. All threads call it.
-template <class Each>
-__device__ __forceinline__ void select_top(uint64_t own, uint32_t n, uint64_t* s_own, uint64_t* s_list, uint32_t* s_count,
-                                           uint64_t* out, Each each) {
-    const uint32_t tid = threadIdx.x;
-    uint64_t* s_bound = s_own + kThreads;
-    s_own[tid] = own;
-    if (tid == 0) {
-        *s_bound = 1;  // any key
-        *s_count = 0;
+// A bound that n to kAccept(n) of the 256 keys in LDS reach, or 1 where fewer than n are there (0: none).
+// Every wavefront works it out for itself, bit by bit from the highest: by the keys' logits alone, and on
+// into their indices only where more than kAccept(n) share the last logit.
+__device__ __forceinline__ constexpr uint32_t kAccept(uint32_t n) { return n + n / 2; }
+__device__ __forceinline__ uint64_t find_bound(const uint64_t* s_own, uint32_t n) {
+    uint64_t k[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) k[i] = s_own[64 * i + (threadIdx.x & 63)];
+    uint32_t count = 0, hi = 0;
+    for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+        uint32_t reach = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) reach += __popcll(__ballot((uint32_t)(k[i] >> 32) >= (hi | bit)));
+        if (reach < n) continue;
+        hi |= bit;
+        count = reach;
+        if (count <= kAccept(n)) break;
     }
-    if (tid < n) out[tid] = 0;
-    __syncthreads();
-    uint32_t above = 0;
-    for (int i = 0; i < kThreads; i++) above += s_own[i] > own;
-    if (own && above == n - 1) *s_bound = own;  // keys are unique: one thread at most
-    __syncthreads();
-    const uint64_t bound = *s_bound;
-    if (own >= bound)
-        each(bound, [&](uint64_t k) {
-            if (k >= bound) s_list[atomicAdd(s_count, 1u)] = k;
-        });
-    __syncthreads();
-    const uint32_t count = *s_count;
+    uint64_t bound = (uint64_t)hi << 32;
+    if (!count) return 1;
+    for (uint64_t bit = 0x80000000u; bit && count > kAccept(n); bit >>= 1) {
+        uint32_t reach = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) reach += __popcll(__ballot(k[i] >= (bound | bit)));
+        if (reach < n) continue;
+        bound |= bit;
+        count = reach;
+    }
+    return bound;
+}
+
+// The n largest of the keys in s_list into out[0, n), in descending order (0 where there are fewer).
+__device__ __forceinline__ void order_top(const uint64_t* s_list, uint32_t count, uint32_t n, uint64_t* out) {
+    const uint32_t tid = threadIdx.x;
     for (uint32_t i = tid; i < count; i += kThreads) {
         const uint64_t k = s_list[i];
         uint32_t rank = 0;
+#pragma unroll 4
         for (uint32_t j = 0; j < count; j++) rank += s_list[j] > k;
         if (rank < n) out[rank] = k;
     }
+    if (tid >= count && tid < n) out[tid] = 0;
     __syncthreads();
 }
 
-// op over the workgroup, on every thread; s_red: 4 floats, free again after a barrier
-template <class F>
-__device__ __forceinline__ float block_reduce(float v, F op, float* s_red) {
-    v = wave_allreduce(v, op);
+// s, c and a summed over the workgroup, on every thread
+__device__ __forceinline__ void block_sums(float& s, float& c, float& a, float (*s_sums)[3]) {
+    const uint32_t wave = threadIdx.x >> 6;
+    s = wave_allreduce(s, OpAdd{});
+    c = wave_allreduce(c, OpAdd{});
+    a = wave_allreduce(a, OpAdd{});
+    if ((threadIdx.x & 63) == 0) {
+        s_sums[wave][0] = s;
+        s_sums[wave][1] = c;
+        s_sums[wave][2] = a;
+    }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) s_red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return op(op(s_red[0], s_red[1]), op(s_red[2], s_red[3]));
+    s = (s_sums[0][0] + s_sums[1][0]) + (s_sums[2][0] + s_sums[3][0]);
+    c = (s_sums[0][1] + s_sums[1][1]) + (s_sums[2][1] + s_sums[3][1]);
+    a = (s_sums[0][2] + s_sums[1][2]) + (s_sums[2][2] + s_sums[3][2]);
 }
 
 // What a row's outputs are, from its joined state and keys in LDS. Called by all threads.
 __device__ __forceinline__ void write_row(const LogprobsParams& p, uint32_t row, float m, float s, float c, float a, float t,
                                           const uint64_t* s_keys) {
     const uint32_t tid = threadIdx.x;
-    const bool none = !(fabsf(m) < INFINITY);  // NaN, +inf, or nothing but -inf
+    const bool none = !(fabsf(m) < INFINITY && s < INFINITY);  // NaN (in s), +inf, or nothing but -inf
     const float rest = (c - 1.0f) + s, log_z = log1pf(rest);
     if (tid == 0) {
         // (t is NaN where no segment held the target)
@@ -117,8 +134,8 @@ __device__ __forceinline__ void write_row(const LogprobsParams& p, uint32_t row,
 
 template <int PER, bool VEC>
 __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(LogprobsParams p) {
-    __shared__ uint64_t s_own[kThreads + 1], s_list[PER * kTop], s_keys[kTop];
-    __shared__ float s_red[4];
+    __shared__ uint64_t s_own[kThreads], s_list[PER * kAccept(kTop)], s_keys[kTop];
+    __shared__ float s_max[4], s_sums[4][3];
     __shared__ uint32_t s_count;
     const uint32_t tid = threadIdx.x, row = blockIdx.x / p.n_segs, seg = blockIdx.x % p.n_segs;
     const uint32_t first = seg * (PER * kThreads);
@@ -145,43 +162,53 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(LogprobsParams 
 #pragma unroll
         for (int e = 0; e < PER; e++) v[e] = id_of(e) < p.vocab ? x[id_of(e)] : -INFINITY;
     }
-    float mx = -INFINITY;
-    bool odd = false;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        mx = fmaxf(mx, v[e]);
-        odd = odd || !(v[e] < INFINITY);
-    }
-    if (odd) mx = INFINITY;  // NaN or +inf
-    const float m = block_reduce(mx, OpMax{}, s_red);
-    float s = 0.0f, c = 0.0f, a = 0.0f;
-    if (fabsf(m) < INFINITY) {  // uniform
-#pragma unroll
-        for (int e = 0; e < PER; e++) {
-            const float d = fmaxf(v[e] - m, -200.0f);  // exp(-200) is 0 here, and 0 * -200 is 0 where 0 * -inf is not
-            const float w = fast_exp2(d * kLog2e);
-            a = __builtin_fmaf(d, w, a);
-            s += v[e] == m ? 0.0f : w;
-            c += v[e] == m ? 1.0f : 0.0f;
-        }
-        s = block_reduce(s, OpAdd{}, s_red);
-        c = block_reduce(c, OpAdd{}, s_red);
-        a = block_reduce(a, OpAdd{}, s_red);
-    }
-    if (p.top_n) {
-        uint64_t own = 0;
-#pragma unroll
-        for (int e = 0; e < PER; e++)
-            if (id_of(e) < p.vocab) own = kmax(own, key_of(v[e], id_of(e)));
-        select_top(own, p.top_n, s_own, s_list, &s_count, s_keys, [&](uint64_t, auto take) {
-#pragma unroll
-            for (int e = 0; e < PER; e++)
-                if (id_of(e) < p.vocab) take(key_of(v[e], id_of(e)));
-        });
-    }
     const int32_t target = p.logprobs ? p.targets[row] : -1;
     const bool here = target >= 0 && (uint32_t)target < p.vocab && (uint32_t)target - first < PER * kThreads;
     const float t = here ? x[target] : NAN;
+    float mx = -INFINITY;
+    uint32_t at = id_of(0);  // of the thread's largest
+#pragma unroll
+    for (int e = 0; e < PER; e++)
+        if (v[e] > mx) {
+            mx = v[e];
+            at = id_of(e);
+        }
+    s_own[tid] = at < p.vocab ? key_of(mx, at) : 0;
+    const float wave_mx = wave_allreduce(mx, OpMax{});
+    if ((tid & 63) == 0) s_max[tid >> 6] = wave_mx;
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    const float m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+    float s = 0.0f, c = 0.0f, a = 0.0f;
+    if (m == -INFINITY) {  // (uniform) the largest of NaN and -inf is -inf
+#pragma unroll
+        for (int e = 0; e < PER; e++) s = v[e] == v[e] ? s : NAN;
+    } else if (m < INFINITY) {
+        uint32_t equal = 0;
+#pragma unroll
+        for (int e = 0; e < PER; e++) {
+            const float d = v[e] - m, w = fast_exp2(d * kLog2e);
+            a = __builtin_fmaf(fmaxf(d, -200.0f), w, a);  // exp(-200) is 0 here, and 0 * -200 is 0 where 0 * -inf is not
+            s += d == 0.0f ? 0.0f : w;
+            equal += d == 0.0f;
+        }
+        c = (float)equal;
+    }
+    if (p.top_n) {
+        const uint64_t bound = find_bound(s_own, p.top_n);
+        if (s_own[tid] >= bound) {
+            const uint32_t o = (uint32_t)(bound >> 32);
+            const float least = bound == 1 ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+#pragma unroll
+            for (int e = 0; e < PER; e++)
+                if (v[e] >= least && id_of(e) < p.vocab) {
+                    const uint64_t k = key_of(v[e], id_of(e));
+                    if (k >= bound) s_list[atomicAdd(&s_count, 1u)] = k;
+                }
+        }
+    }
+    block_sums(s, c, a, s_sums);
+    if (p.top_n) order_top(s_list, s_count, p.top_n, s_keys);
     if (p.n_segs == 1) {
         write_row(p, row, m, s, c, a, t, s_keys);
         return;
@@ -191,20 +218,43 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(LogprobsParams 
 }
 
 __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobsParams p) {
-    __shared__ uint64_t s_own[kThreads + 1], s_list[kTop * kTop], s_keys[kTop];
-    __shared__ float s_red[4];
+    __shared__ uint64_t s_own[kThreads], s_list[kTop * kAccept(kTop)], s_keys[kTop];
+    __shared__ float s_state[4][2], s_sums[4][3];
     __shared__ uint32_t s_count;
-    const uint32_t tid = threadIdx.x, row = blockIdx.x;
+    const uint32_t tid = threadIdx.x, row = blockIdx.x, n = p.top_n;
+    const uint64_t* keys = p.keys + (uint64_t)row * p.n_segs * n;
+    // The bound comes from every segment's first `depth` keys, 2 n of them at least; at most 256, as more
+    // than one of each are taken from fewer than 2 n segments only.
+    const uint32_t n_keys = p.n_segs * n, depth = n ? min(n, (2 * n + p.n_segs - 1) / p.n_segs) : 0;
+    constexpr int kHeld = 8;  // keys a thread holds; it reads those past 256 * kHeld twice
+    uint64_t held[kHeld];
+    s_own[tid] = 0;
     SegState st{-INFINITY, 0.0f, 0.0f, 0.0f, NAN};
-    const uint64_t* keys = nullptr;
-    if (tid < p.n_segs) {
-        st = p.states[(uint64_t)row * p.n_segs + tid];
-        keys = p.keys + ((uint64_t)row * p.n_segs + tid) * p.top_n;
+    if (tid < p.n_segs) st = p.states[(uint64_t)row * p.n_segs + tid];
+#pragma unroll
+    for (int i = 0; i < kHeld; i++) held[i] = tid + kThreads * i < n_keys ? keys[tid + kThreads * i] : 0;
+    const float wave_m = wave_allreduce(st.m, OpMax{});
+    const float wave_t = wave_allreduce(st.t == st.t ? st.t : -INFINITY, OpMax{});  // one segment holds it, or none
+    const bool wave_has = __any(st.t == st.t);
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    auto sample = [&](uint32_t i, uint64_t k) {
+        const uint32_t seg = i / n, at = i - seg * n;
+        if (at < depth) s_own[seg * depth + at] = k;
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; i++)
+        if (tid + kThreads * i < n_keys) sample(tid + kThreads * i, held[i]);
+    for (uint32_t i = tid + kThreads * kHeld; i < n_keys; i += kThreads) sample(i, keys[i]);
+    if ((tid & 63) == 0) {
+        s_state[tid >> 6][0] = wave_m;
+        s_state[tid >> 6][1] = wave_has ? wave_t : NAN;
     }
-    const float m = block_reduce(st.m, OpMax{}, s_red);
-    float s = 0.0f, c = 0.0f, a = 0.0f;
+    __syncthreads();
+    const float m = fmaxf(fmaxf(s_state[0][0], s_state[1][0]), fmaxf(s_state[2][0], s_state[3][0]));
+    const float t = fmaxf(fmaxf(s_state[0][1], s_state[1][1]), fmaxf(s_state[2][1], s_state[3][1]));  // of those not NaN
+    float s = st.s, c = 0.0f, a = 0.0f;
     if (st.m == m) {
-        s = st.s;
         c = st.c;
         a = st.a;
     } else if (st.m > -INFINITY) {
@@ -212,16 +262,18 @@ __global__ __launch_bounds__(kThreads) void logprobs_join_kernel(LogprobsParams 
         s = z * w;
         a = w * __builtin_fmaf(d, z, st.a);
     }
-    s = block_reduce(s, OpAdd{}, s_red);
-    c = block_reduce(c, OpAdd{}, s_red);
-    a = block_reduce(a, OpAdd{}, s_red);
-    const float t = block_reduce(st.t == st.t ? st.t : -INFINITY, OpMax{}, s_red);  // one segment holds it, or none
-    const float held = block_reduce(st.t == st.t ? 1.0f : 0.0f, OpMax{}, s_red);
-    if (p.top_n)
-        select_top(keys ? keys[0] : 0, p.top_n, s_own, s_list, &s_count, s_keys, [&](uint64_t bound, auto take) {
-            for (uint32_t i = 0; i < p.top_n && keys[i] >= bound; i++) take(keys[i]);
-        });
-    write_row(p, row, m, s, c, a, held > 0.0f ? t : NAN, s_keys);
+    if (n) {
+        const uint64_t bound = find_bound(s_own, n);
+        auto take = [&](uint64_t k) {
+            if (k >= bound) s_list[atomicAdd(&s_count, 1u)] = k;
+        };
+#pragma unroll
+        for (int i = 0; i < kHeld; i++) take(held[i]);
+        for (uint32_t i = tid + kThreads * kHeld; i < n_keys; i += kThreads) take(keys[i]);
+    }
+    block_sums(s, c, a, s_sums);
+    if (n) order_top(s_list, s_count, n, s_keys);
+    write_row(p, row, m, s, c, a, t, s_keys);
 }
 
 }  // namespace

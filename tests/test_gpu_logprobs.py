@@ -241,3 +241,15 @@ def test_a_served_batch(ctx, hip):
         # k and v rows may round to either side of a step of f16 (2^-11 of them) where f32 and f64 projections part:
         # a rare element, 2^-11 of it through softmax and two projections of unit gain
         assert np.all(np.abs(np.concatenate(got[b]) - want) <= 2e-3), b
+
+
+@pytest.mark.parametrize("V,at", [(8193, 8192), (2 ** 19 + 1, 2 ** 19), (70001, 70000), (300, 299)])
+@pytest.mark.parametrize("rest", [0.0, -np.inf])
+def test_nan_alone_in_a_segment(ctx, hip, V, at, rest):
+    """A NaN whose part of the row holds nothing else, or nothing else but -inf, undoes the row all the same."""
+    x = np.random.default_rng(V).standard_normal((2, V)).astype(np.float32)
+    x[1, V // 8192 * 8192:] = rest
+    x[1, at] = np.nan
+    lp, ent, ids, tops = run(ctx, hip, x, np.zeros(2, int), 3)
+    assert np.isfinite([lp[0], ent[0], *tops[0]]).all()
+    assert np.isnan([lp[1], ent[1], *tops[1]]).all() and np.all(ids[1] == -1)
