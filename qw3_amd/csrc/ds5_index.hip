@@ -180,7 +180,7 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
             if (y - from < work) break;
             from += work;
         }
-        pb_locate(seq(c.b), group, y - from, snap, whole != 0, c.j, c.k);
+        pb_locate(seq(c.b), group, y - from, snap, pb_lead(total, share, group), whole != 0, c.j, c.k);
         line = c.kvh * per_head + from + pb_before(seq(c.b), group, c.j);
         return c;
     };

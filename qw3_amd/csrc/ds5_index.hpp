@@ -203,13 +203,15 @@ DS5_HD uint32_t af_row_splits(uint32_t lim, uint32_t chunk) { return lim / chunk
 // below its last token's. The batch's work is one line: for each kv head, each sequence, each
 // tile in the order last, first, last but one, second, ... (a pair of them costs the same for
 // every pair), its positions. Workgroup w of n takes the part from w / n to (w + 1) / n of it.
-// Work is counted in positions * group, a tile's being its positions (taken as if every tile
-// were full) and kPbTileCost more, twice for the tiles of sequences of more than kPbNarrow rows
-// (64 positions of a tile of 128 rows take 1.5 us, of one of 32 rows 0.7 where the caches'
-// rows arrive in time; beginning and ending a tile 8 and 5). A cut inside a tile falls on a multiple of kPbUnit
-// positions of it, or on the tile's start or end where that is no further than `snap`.
+// Work is counted in half positions * group for the tiles of sequences of at most kPbNarrow rows
+// and in fifths for the others (64 positions measured 0.5 .. 0.7 us and 1.3 .. 1.5), a tile's being
+// its positions (taken as if every tile were full) and before them kPbTileCost for beginning and
+// ending it (10 us and 12). A workgroup whose part begins inside a tile, or ends there, pays that
+// as every other does; what counts is the tiles that it begins after another, so the cost lies at
+// the tile's start, and cuts there fall on the start. A cut further on falls on a multiple of
+// kPbUnit positions, or on the tile's start or end where that is no further than `snap`.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 512, kPbPiece = 192;
+constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 2304, kPbPiece = 384;
 
 struct PbSeq {
     uint32_t n, before;  // new tokens, and the tokens before them
@@ -222,13 +224,13 @@ struct PbCut {
 };
 
 DS5_HD uint32_t pb_tiles(PbSeq s, uint32_t group) { return (s.n * group + kPbRows - 1) / kPbRows; }
-DS5_HD uint32_t pb_weight(PbSeq s, uint32_t group) { return s.n * group > kPbNarrow ? 2 : 1; }
+DS5_HD uint32_t pb_weight(PbSeq s, uint32_t group) { return s.n * group > kPbNarrow ? 5 : 2; }
 DS5_HD uint64_t pb_tile_work(PbSeq s, uint32_t group, uint32_t tile) {
-    return pb_weight(s, group) * ((uint64_t)group * ((uint64_t)s.before + kPbTileCost) + (uint64_t)kPbRows * (tile + 1));
+    return (uint64_t)group * kPbTileCost + pb_weight(s, group) * ((uint64_t)group * s.before + (uint64_t)kPbRows * (tile + 1));
 }
 DS5_HD uint64_t pb_seq_work(PbSeq s, uint32_t group) {
     const uint64_t nt = pb_tiles(s, group);
-    return pb_weight(s, group) * (nt * group * ((uint64_t)s.before + kPbTileCost) + kPbRows / 2 * nt * (nt + 1));
+    return nt * group * kPbTileCost + pb_weight(s, group) * (nt * group * s.before + kPbRows / 2 * nt * (nt + 1));
 }
 DS5_HD uint32_t pb_tile_at(uint32_t j, uint32_t nt) { return j % 2 ? j / 2 : nt - 1 - j / 2; }
 DS5_HD PbTile pb_tile(PbSeq s, uint32_t group, uint32_t tile) {
@@ -257,7 +259,7 @@ DS5_HD uint64_t pb_divide(uint64_t x, uint64_t d, uint64_t& r) {
     return q;
 }
 // The cut at y of a sequence's work: tile j of its order (j may be one past the last), position k.
-DS5_HD void pb_locate(PbSeq s, uint32_t group, uint64_t y, uint64_t snap, bool whole, uint32_t& j, uint32_t& k) {
+DS5_HD void pb_locate(PbSeq s, uint32_t group, uint64_t y, uint64_t snap, uint64_t lead, bool whole, uint32_t& j, uint32_t& k) {
     const uint32_t nt = pb_tiles(s, group);
     const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
     uint64_t off;
@@ -274,13 +276,13 @@ DS5_HD void pb_locate(PbSeq s, uint32_t group, uint64_t y, uint64_t snap, bool w
         j += off * 2 >= w;
         return;
     }
-    if (off < snap) return;
+    if (off < snap || off <= lead) return;
     if (w - off < snap) {
         j++;
         return;
     }
     const uint32_t kv = pb_tile(s, group, tile).kv;
-    k = umin((uint32_t)((double)kv * (double)off / (double)w), kv - 1) / kPbUnit * kPbUnit;
+    k = umin((uint32_t)((double)kv * (double)(off - lead) / (double)(w - lead)), kv - 1) / kPbUnit * kPbUnit;
 }
 // The cut before workgroup w of n on a line of `work` (below 2^53): rounded, but never backwards as w
 // grows, and the same wherever it is worked out. part: 1.0 / n.
@@ -298,7 +300,13 @@ DS5_HD uint64_t pb_snap(uint64_t work, double part, uint32_t group) {
     const uint64_t share = (uint64_t)((double)work * part * 0.0625), least = (uint64_t)group * (kPbUnit / 2);
     return share > least ? share : least;
 }
-// The workgroups that share a line of work: kPbPiece positions of a tile each at least, and the same number
+// A tile's cost that lies before its positions; of tiles that several workgroups share, no more than
+// leaves each of them some.
+DS5_HD uint64_t pb_lead(uint64_t work, double part, uint32_t group) {
+    const uint64_t half = (uint64_t)((double)work * part * 0.5), cost = (uint64_t)group * kPbTileCost;
+    return half < cost ? half : cost;
+}
+// The workgroups that share a line of work: kPbPiece of a row's work each at least, and the same number
 // for each kv head where there are enough, so that no workgroup ends one head's tile to begin another's.
 DS5_HD uint32_t pb_workgroups(uint64_t work, uint32_t group, uint32_t heads, uint32_t grid) {
     const double n = (double)work / ((double)group * kPbPiece);

@@ -657,7 +657,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                     continue;
                 }
                 uint32_t j, k;
-                ds5idx::pb_locate(seq(b), G, y - f, snap, p.whole, j, k);
+                ds5idx::pb_locate(seq(b), G, y - f, snap, ds5idx::pb_lead(total, share, G), p.whole, j, k);
                 (c ? s_walk.stop : s_walk.at) = ds5idx::PbCut{h, b, j, k};
                 if (c == 0) s_walk.line = h * per_head + f + ds5idx::pb_before(seq(b), G, j);
                 break;
@@ -1150,13 +1150,13 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     p.page_shift = (b.page_size & (b.page_size - 1)) == 0 ? (uint32_t)__builtin_ctz(b.page_size) : 0;
     const uint64_t rows = (uint64_t)b.n_tokens * p.group, tiles = rows / kRows + std::min<uint64_t>(b.n_seqs, b.n_tokens);
     // the work that the plan counts, at most: below 2^53
-    if (2.0 * b.n_kv_heads * tiles * ((double)p.group * ((double)b.max_seq_len + ds5idx::kPbTileCost) + rows + kRows) >= 9007199254740992.0)
+    if ((double)b.n_kv_heads * tiles * ((double)p.group * (5.0 * b.max_seq_len + ds5idx::kPbTileCost) + 5.0 * (rows + kRows)) >= 9007199254740992.0)
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "paged_attention: batch too large");
     // Up to 256 positions a workgroup's eight wavefronts take a tile in one go: none is cut then,
     // and nothing merged. (Nor without the context's memory for parts.)
     p.whole = !ctx->split_buf || b.max_seq_len <= 256;
     const uint64_t most =
-        b.n_kv_heads * tiles * (p.whole ? 1 : 2 * ((uint64_t)b.max_seq_len + ds5idx::kPbTileCost) / ds5idx::kPbPiece + 1);
+        b.n_kv_heads * tiles * (p.whole ? 1 : (5ull * b.max_seq_len + ds5idx::kPbTileCost) / ds5idx::kPbPiece + 1);
     const uint32_t cus = std::min(kMaxGrid, ctx->cu_count > 0 ? (uint32_t)ctx->cu_count : kMaxGrid);
     const dim3 grid((uint32_t)std::min<uint64_t>(most, cus)), block(kThreads);
     if (!p.whole) {
