@@ -4,19 +4,24 @@ import numpy as np
 
 class Batch:
     """Sequences of ctx[b] cached and new[b] new tokens, their pages a random draw from a pool that has
-    `spare` pages more; pool rows that no sequence holds are NaN."""
+    `spare` pages more; pool rows that no sequence holds are NaN. pool: the pages come from a pool of this many
+    instead, any of them as often as it is drawn."""
 
-    def __init__(self, seed, ctx, new, hq, hkv, d, page=16, spare=3, behind=0, q_f16=False, std=1.0):
+    def __init__(self, seed, ctx, new, hq, hkv, d, page=16, spare=3, behind=0, q_f16=False, std=1.0, pool=0):
         g = self.g = np.random.default_rng([seed, len(ctx), sum(ctx), sum(new)])
         self.ctx, self.new, self.hq, self.hkv, self.d, self.page = list(ctx), list(new), hq, hkv, d, page
         self.lens = [a + b for a, b in zip(ctx, new)]
         self.T, self.rows = sum(new), sum(new) + behind
         pages = [-(-n // page) for n in self.lens]
-        self.n_pages, self.max_pages = sum(pages) + spare, max(max(pages), 1) + 1
+        self.n_pages, self.max_pages = sum(pages) + spare if not pool else pool, max(max(pages), 1) + 1
         perm, at = g.permutation(self.n_pages), 0
         self.table = np.full((len(ctx), self.max_pages), -7, np.int32)  # out of range: never used
         self.kp, self.vp = (np.full((hkv, self.n_pages * page, d), np.nan, np.float16) for _ in range(2))
-        for b, n in enumerate(pages):
+        if pool:
+            self.kp, self.vp = ((g.standard_normal((hkv, pool * page, d)) * std).astype(np.float16) for _ in range(2))
+            for b, n in enumerate(pages):
+                self.table[b, :n] = g.integers(0, pool, n)
+        for b, n in enumerate(pages if not pool else ()):
             self.table[b, :n] = perm[at:at + n]
             at += n
             s = self.slots(b, self.lens[b])

@@ -83,6 +83,13 @@ def test_paged_attention_many_sequences(ctx, hip):
     check_attention(ctx, hip, Batch(2, g.integers(0, 60, 1024).tolist(), g.integers(0, 3, 1024).tolist(), 4, 1, 64))
 
 
+@pytest.mark.parametrize("new,q_f16", [(1, False), (33, True)])
+def test_paged_attention_long_parts(ctx, hip, new, q_f16):
+    """More tiles than workgroups, of 24000 positions each: parts of a tile longer than the 16384 positions
+    whose pages a workgroup holds at a time. (Wide and narrow tiles; the sequences share their pages.)"""
+    check_attention(ctx, hip, Batch(9, [24000 - 7 * i for i in range(34)], [new] * 34, 8, 8, 64, 48, pool=100, q_f16=q_f16), q_f16)
+
+
 @pytest.mark.parametrize("std", [1e-3, 30.0])
 def test_paged_attention_small_and_large_scores(ctx, hip, std):
     """q and the caches scaled: nearly uniform weights, and weights of one position alone."""
