@@ -173,14 +173,14 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
     auto cut = [&](uint32_t w) {
         if (w == n_wg) return PbCut{n_kv_heads, 0, 0, 0};
         uint64_t y;
-        PbCut c{(uint32_t)pb_divide(pb_cut_at(total, w, n_wg, share), per_head, y), 0, 0, 0};
+        PbCut c{pb_divide(pb_cut_at(total, w, n_wg, share), per_head, y), 0, 0, 0};
         uint64_t from = 0;
         for (;; c.b++) {
             const uint64_t work = n[c.b] ? pb_seq_work(seq(c.b), group) : 0;
             if (y - from < work) break;
             from += work;
         }
-        pb_locate(seq(c.b), group, y - from, snap, pb_lead(total, share, group), whole != 0, c.j, c.k);
+        pb_locate(seq(c.b), group, 1.0 / group, y - from, snap, pb_lead(total, share, group), whole != 0, c.j, c.k);
         line = c.kvh * per_head + from + pb_before(seq(c.b), group, c.j);
         return c;
     };
@@ -191,7 +191,7 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
         bool at_end = false;
         for (; !at_end && pb_next(at, stop, n_seqs, n_kv_heads, group, seq, at_end); at.j++, at.k = 0) {
             const uint32_t ti = pb_tile_at(at.j, pb_tiles(seq(at.b), group));
-            const PbTile t = pb_tile(seq(at.b), group, ti);
+            const PbTile t = pb_tile(seq(at.b), group, 1.0 / group, ti);
             const uint32_t end = at_end ? stop.k : t.kv;
             const uint64_t tile_end = line + pb_tile_work(seq(at.b), group, ti);
             if (count < max) {

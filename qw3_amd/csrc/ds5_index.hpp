@@ -233,9 +233,11 @@ DS5_HD uint64_t pb_seq_work(PbSeq s, uint32_t group) {
     return nt * group * kPbTileCost + pb_weight(s, group) * (nt * group * s.before + kPbRows / 2 * nt * (nt + 1));
 }
 DS5_HD uint32_t pb_tile_at(uint32_t j, uint32_t nt) { return j % 2 ? j / 2 : nt - 1 - j / 2; }
-DS5_HD PbTile pb_tile(PbSeq s, uint32_t group, uint32_t tile) {
+// x / d with inv = 1.0 / d: the floor of (x + 1/2) / d, which is half of 1 / d or more away from every integer.
+DS5_HD uint32_t pb_over(uint32_t x, double inv) { return (uint32_t)(((double)x + 0.5) * inv); }
+DS5_HD PbTile pb_tile(PbSeq s, uint32_t group, double inv_group, uint32_t tile) {
     const uint32_t all = s.n * group, row0 = tile * kPbRows, end = umin(all, row0 + kPbRows);
-    return PbTile{row0, end - row0, s.before + (end - 1) / group + 1};
+    return PbTile{row0, end - row0, s.before + pb_over(end - 1, inv_group) + 1};
 }
 // The work before the j-th tile of a sequence's order.
 DS5_HD uint64_t pb_before(PbSeq s, uint32_t group, uint32_t j) {
@@ -243,11 +245,20 @@ DS5_HD uint64_t pb_before(PbSeq s, uint32_t group, uint32_t j) {
     const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
     return j / 2 * pair + (j % 2 ? pb_tile_work(s, group, nt - 1 - j / 2) : 0);
 }
-// x = q * d + r. (In f64, whose quotient is at most one off for x below 2^53: a 64-bit integer division
-// takes several times as long on the device.)
-DS5_HD uint64_t pb_divide(uint64_t x, uint64_t d, uint64_t& r) {
-    uint64_t q = (uint64_t)((double)x / (double)d);
-    int64_t left = (int64_t)(x - q * d);
+// 1 / d for d from 1 on, to 2^-44 or better: the device's estimate (to 2^-22) and one step of Newton's method.
+// (A division of doubles takes several times as long there, one of 64-bit integers longer still.)
+DS5_HD double pb_inverse(double d) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const double r = __builtin_amdgcn_rcp(d);
+    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+#else
+    return 1.0 / d;
+#endif
+}
+// x = q * d + r, with x below 2^53 and q below 2^32: the quotient in f64 is at most one off.
+DS5_HD uint32_t pb_divide(uint64_t x, uint64_t d, uint64_t& r) {
+    uint32_t q = (uint32_t)((double)x * pb_inverse((double)d));
+    int64_t left = (int64_t)(x - (uint64_t)q * d);
     if (left < 0) {
         q--;
         left += (int64_t)d;
@@ -259,11 +270,11 @@ DS5_HD uint64_t pb_divide(uint64_t x, uint64_t d, uint64_t& r) {
     return q;
 }
 // The cut at y of a sequence's work: tile j of its order (j may be one past the last), position k.
-DS5_HD void pb_locate(PbSeq s, uint32_t group, uint64_t y, uint64_t snap, uint64_t lead, bool whole, uint32_t& j, uint32_t& k) {
+DS5_HD void pb_locate(PbSeq s, uint32_t group, double inv_group, uint64_t y, uint64_t snap, uint64_t lead, bool whole, uint32_t& j, uint32_t& k) {
     const uint32_t nt = pb_tiles(s, group);
     const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
     uint64_t off;
-    j = (uint32_t)pb_divide(y, pair, off) * 2;
+    j = pb_divide(y, pair, off) * 2;
     const uint64_t heavy = pb_tile_work(s, group, pb_tile_at(j, nt));
     if (j + 1 < nt && off >= heavy) {
         j++;
@@ -281,8 +292,8 @@ DS5_HD void pb_locate(PbSeq s, uint32_t group, uint64_t y, uint64_t snap, uint64
         j++;
         return;
     }
-    const uint32_t kv = pb_tile(s, group, tile).kv;
-    k = umin((uint32_t)((double)kv * (double)(off - lead) / (double)(w - lead)), kv - 1) / kPbUnit * kPbUnit;
+    const uint32_t kv = pb_tile(s, group, inv_group, tile).kv;
+    k = umin((uint32_t)((double)kv * (double)(off - lead) * pb_inverse((double)(w - lead))), kv - 1) / kPbUnit * kPbUnit;
 }
 // The cut before workgroup w of n on a line of `work` (below 2^53): rounded, but never backwards as w
 // grows, and the same wherever it is worked out. part: 1.0 / n.
@@ -309,7 +320,7 @@ DS5_HD uint64_t pb_lead(uint64_t work, double part, uint32_t group) {
 // The workgroups that share a line of work: kPbPiece of a row's work each at least, and the same number
 // for each kv head where there are enough, so that no workgroup ends one head's tile to begin another's.
 DS5_HD uint32_t pb_workgroups(uint64_t work, uint32_t group, uint32_t heads, uint32_t grid) {
-    const double n = (double)work / ((double)group * kPbPiece);
+    const double n = (double)work * pb_inverse((double)group * kPbPiece);
     const uint32_t all = n >= (double)grid ? grid : n < 1.0 ? 1 : (uint32_t)n;
     return all > heads ? all / heads * heads : all;
 }

@@ -168,7 +168,7 @@ struct MergeDesc {
 struct AttnParams {
     PagedAttentionLaunch a;
     uint32_t group;
-    uint32_t page_shift;  // log2 of page_size where it is a power of two, else 0
+    double inv_group, inv_page;  // 1 / group, 1 / page_size
     bool whole;        // no tile is cut
     float* part_o;     // [2 * workgroups, kRows, D]: slot 2 w the part that workgroup w continues, 2 w + 1 the one it begins
     float2* part_ml;   // [2 * workgroups, kRows]: reference and sum
@@ -597,10 +597,12 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     {
         const PagedBatch& bt = p.a.batch;
         const uint32_t G = p.group;
-        constexpr uint32_t N = kMaxSeqs / kThreads;  // sequences a thread, consecutive ones
+        // The workgroup's two halves do the same for the part's two cuts: a thread's sequences are consecutive ones.
+        constexpr uint32_t kHalf = kThreads / 2;
+        const uint32_t cut = uniform(tid / kHalf), i = tid % kHalf, N = (n_seqs + kHalf - 1) / kHalf, b0 = i * N;
         uint64_t mine = 0;
 #pragma unroll 1
-        for (uint32_t b = tid * N; b < min(tid * N + N, n_seqs); b++) {
+        for (uint32_t b = b0; b < min(b0 + N, n_seqs); b++) {
             const int64_t s0 = bt.starts[b], s1 = bt.starts[b + 1], len = bt.seq_lens[b];
             const int64_t c0 = max(s0, (int64_t)0), c1 = min(s1, (int64_t)bt.n_tokens);
             const uint32_t n = c1 > c0 ? (uint32_t)(c1 - c0) : 0;
@@ -611,21 +613,20 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             mine += ds5idx::pb_seq_work(seq(b), G);
         }
         uint64_t upto = mine;  // inclusive over the wavefront
-        if (n_seqs > N) {
+        if (n_seqs > 1) {
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const uint64_t y = __shfl_up(upto, o, 64);
                 if ((int)lane >= o) upto += y;
             }
         }
-        if (lane == 63) s_scan[wave] = n_seqs > N ? upto : 0;
-        if (n_seqs <= N && tid == 0) s_scan[0] = mine;
+        if (lane == 63 || n_seqs == 1) s_scan[wave] = n_seqs > 1 ? upto : uniform64(mine);
         __syncthreads();
         uint64_t from = upto - mine, per_head = 0;
 #pragma unroll
-        for (uint32_t w = 0; w < (uint32_t)kWaves; w++) {
-            const uint64_t x = s_scan[w];
-            from += w < wave ? x : 0;
+        for (uint32_t w = 0; w < (uint32_t)kWaves / 2; w++) {
+            const uint64_t x = s_scan[cut * (kWaves / 2) + w];
+            from += w < wave % (kWaves / 2) ? x : 0;
             per_head += x;
         }
         per_head = uniform64(per_head);
@@ -645,24 +646,21 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             s_walk.at_end = 0;
             if (wg + 1 == n_wg) s_walk.stop = ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0};
         }
-#pragma unroll 1
-        for (uint32_t c = 0; c < (wg + 1 < n_wg ? 2u : 1u); c++) {
-            uint64_t y, f = from;
-            const uint32_t h = (uint32_t)ds5idx::pb_divide(ds5idx::pb_cut_at(total, wg + c, n_wg, share), per_head, y);
-            if (y < from || y - from >= mine) continue;
-            for (uint32_t b = tid * N;; b++) {
+        uint64_t y;
+        const uint32_t h = ds5idx::pb_divide(ds5idx::pb_cut_at(total, wg + cut, n_wg, share), per_head, y);
+        if (y >= from && y - from < mine && wg + cut < n_wg)
+            for (uint32_t b = b0;; b++) {
                 const uint64_t work = ds5idx::pb_seq_work(seq(b), G);
-                if (y - f >= work) {
-                    f += work;
+                if (y - from >= work) {
+                    from += work;
                     continue;
                 }
                 uint32_t j, k;
-                ds5idx::pb_locate(seq(b), G, y - f, snap, ds5idx::pb_lead(total, share, G), p.whole, j, k);
-                (c ? s_walk.stop : s_walk.at) = ds5idx::PbCut{h, b, j, k};
-                if (c == 0) s_walk.line = h * per_head + f + ds5idx::pb_before(seq(b), G, j);
+                ds5idx::pb_locate(seq(b), G, p.inv_group, y - from, snap, ds5idx::pb_lead(total, share, G), p.whole, j, k);
+                (cut ? s_walk.stop : s_walk.at) = ds5idx::PbCut{h, b, j, k};
+                if (cut == 0) s_walk.line = h * per_head + from + ds5idx::pb_before(seq(b), G, j);
                 break;
             }
-        }
     }
     __syncthreads();
 
@@ -673,7 +671,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             w.more = ds5idx::pb_next(w.at, w.stop, n_seqs, p.a.batch.n_kv_heads, p.group, seq, at_end);
             if (w.more) {
                 const ds5idx::PbSeq sq = seq(w.at.b);
-                w.tile = ds5idx::pb_tile(sq, p.group, ds5idx::pb_tile_at(w.at.j, ds5idx::pb_tiles(sq, p.group)));
+                w.tile = ds5idx::pb_tile(sq, p.group, p.inv_group, ds5idx::pb_tile_at(w.at.j, ds5idx::pb_tiles(sq, p.group)));
                 w.start = s_start[w.at.b];
                 w.before = sq.before;
                 w.poison = s_before[w.at.b] & kPoison;
@@ -706,17 +704,17 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             const PagedBatch& bt = p.a.batch;
             // ---- this wavefront's 32 query rows
             const uint32_t row = row0 + min(32 * rg + r32, rows - 1);
-            t.lim = before + row / G;
-            const uint32_t lim_lo = uniform(before + (row0 + min(32 * rg, rows - 1)) / G);
-            const uint32_t lim_hi = uniform(before + (row0 + min(32 * rg + 31, rows - 1)) / G);
+            const uint32_t token = ds5idx::pb_over(row, p.inv_group);
+            t.lim = before + token;
+            const uint32_t lim_lo = uniform(before + ds5idx::pb_over(row0 + min(32 * rg, rows - 1), p.inv_group));
+            const uint32_t lim_hi = uniform(before + ds5idx::pb_over(row0 + min(32 * rg + 31, rows - 1), p.inv_group));
             typename A::Query query;
             const uint32_t start = uniform(wk.start);
             if constexpr (narrow)
-                A::fetch_q(query, p, ((uint64_t)(start + row / G) * bt.n_q_heads + kvh * G + row % G) * D + 8 * h);
+                A::fetch_q(query, p, ((uint64_t)(start + token) * bt.n_q_heads + kvh * G + (row - token * G)) * D + 8 * h);
             else {
-                const double inv_g = 1.0 / (double)G;  // x / G is the floor of (x + 1/2) / G, which f64 keeps apart from an integer
                 A::stage_q(lds_addr(s_kv) + A::AREA / 2, p.a.q, wave, lane, [&](uint32_t r) -> uint64_t {
-                    const uint32_t packed = row0 + min(r, rows - 1), token = (uint32_t)(((double)packed + 0.5) * inv_g);
+                    const uint32_t packed = row0 + min(r, rows - 1), token = ds5idx::pb_over(packed, p.inv_group);
                     return (uint64_t)(start + token) * bt.n_q_heads + kvh * G + (packed - token * G);
                 });
             }
@@ -735,7 +733,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                 last = (to - from - 1) / 16;
 #pragma unroll 1
                 for (uint32_t i = tid; i <= last; i += kThreads) {
-                    const uint32_t pos = from + 16 * i, page = p.page_shift ? pos >> p.page_shift : pos / page_size;
+                    const uint32_t pos = from + 16 * i, page = ds5idx::pb_over(pos, p.inv_page);
                     const uint32_t pg = (uint32_t)table[page];  // (a page out of range: page 0, and the rows that attend it are NaN)
                     s_groups[i] = (pg < bt.n_pages ? pg : 0) * (page_size / 16) + (pos - page * page_size) / 16;
                     if (pg >= bt.n_pages) atomicMin(&s_bad, pos);
@@ -906,12 +904,12 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                     }
                 }
                 if (odd && lane == 0) s_odd = 1;
-                float zero = 0.0f;  // (NaN where O holds an infinity or NaN)
+                float zero[4] = {};  // (NaN where O holds an infinity or NaN)
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) zero = __builtin_fmaf(t.O[dt][e], 0.0f, zero);
-                if (__ballot(!(zero == 0.0f)) != 0 && lane == 0) s_broken = 1;
+                    for (int e = 0; e < 16; e++) zero[e % 4] = __builtin_fmaf(t.O[dt][e], 0.0f, zero[e % 4]);
+                if (__ballot(!((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f)) != 0 && lane == 0) s_broken = 1;
                 __syncthreads();
                 if (careful || uniform(s_broken) == 0) break;
                 careful = true;
@@ -953,7 +951,6 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             // a row's D / 4 columns to as many threads, kThreads / CH rows at a time
             constexpr uint32_t CH = A::CH, PER = kThreads / CH;
             const uint32_t c = here(tid) % CH, stride = narrow ? 2 * HALF : 8 * HALF;
-            const double inv_g = 1.0 / (double)G;  // x / G is the floor of (x + 1/2) / G, which f64 keeps apart from an integer
             auto fold = [&](uint32_t r, uint32_t w0, float& M, float& L, f32x4& o, auto parts) {
                 constexpr uint32_t N = decltype(parts)::value, STEP = kWaves / N;
                 float mw[N], f[N];
@@ -979,7 +976,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                 f32x4 o;
                 if constexpr (narrow) fold(rr, 0, M, L, o, std::integral_constant<uint32_t, kWaves>{});
                 else fold(rr & 31, rr >> 5, M, L, o, std::integral_constant<uint32_t, 2>{});
-                const uint32_t packed = row0 + rr, token = (uint32_t)(((double)packed + 0.5) * inv_g), pos = before + token;
+                const uint32_t packed = row0 + rr, token = ds5idx::pb_over(packed, p.inv_group), pos = before + token;
                 if (any_odd) {
                     const PagedBatch& bt = p.a.batch;
                     o = add_odd_values(p.a.v_pool + (uint64_t)kvh * bt.n_pages * bt.page_size * D,
@@ -1147,7 +1144,8 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     AttnParams p{};
     p.a = a;
     p.group = b.n_q_heads / b.n_kv_heads;
-    p.page_shift = (b.page_size & (b.page_size - 1)) == 0 ? (uint32_t)__builtin_ctz(b.page_size) : 0;
+    p.inv_group = 1.0 / p.group;
+    p.inv_page = 1.0 / b.page_size;
     const uint64_t rows = (uint64_t)b.n_tokens * p.group, tiles = rows / kRows + std::min<uint64_t>(b.n_seqs, b.n_tokens);
     // the work that the plan counts, at most: below 2^53
     if ((double)b.n_kv_heads * tiles * ((double)p.group * (5.0 * b.max_seq_len + ds5idx::kPbTileCost) + 5.0 * (rows + kRows)) >= 9007199254740992.0)
