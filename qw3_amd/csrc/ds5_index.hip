@@ -162,26 +162,26 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
                             uint32_t grid, int whole, uint32_t max, uint32_t* out) {
     using namespace ds5idx;
     auto seq = [&](uint32_t b) { return PbSeq{n[b], before[b]}; };
-    uint64_t per_head = 0;
+    double per_head = 0;
     for (uint32_t b = 0; b < n_seqs; b++) per_head += n[b] ? pb_seq_work(seq(b), group) : 0;
-    const uint64_t total = per_head * n_kv_heads;
-    if (!total) return 0;
+    const double total = per_head * n_kv_heads;
+    if (total == 0) return 0;
     const uint32_t n_wg = whole ? grid : pb_workgroups(total, group, n_kv_heads, grid);
-    const double share = 1.0 / (double)n_wg;
-    const uint64_t snap = pb_snap(total, share, group);
-    uint64_t line = 0;
+    const double share = pb_inverse(n_wg);
+    const double snap = pb_snap(total, share, group);
+    double line = 0;
     auto cut = [&](uint32_t w) {
         if (w == n_wg) return PbCut{n_kv_heads, 0, 0, 0};
-        uint64_t y;
+        double y, from = 0;
         PbCut c{pb_divide(pb_cut_at(total, w, n_wg, share), per_head, y), 0, 0, 0};
-        uint64_t from = 0;
         for (;; c.b++) {
-            const uint64_t work = n[c.b] ? pb_seq_work(seq(c.b), group) : 0;
+            const double work = n[c.b] ? pb_seq_work(seq(c.b), group) : 0;
             if (y - from < work) break;
             from += work;
         }
-        pb_locate(seq(c.b), group, 1.0 / group, y - from, snap, pb_lead(total, share, group), whole != 0, c.j, c.k);
-        line = c.kvh * per_head + from + pb_before(seq(c.b), group, c.j);
+        const PbPlace at = pb_locate(seq(c.b), group, 1.0 / group, y - from, snap, pb_lead(total, share, group), whole != 0);
+        c.j = at.j, c.k = at.k;
+        line = c.kvh * per_head + from + at.at;
         return c;
     };
     uint32_t count = 0;
@@ -193,7 +193,7 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
             const uint32_t ti = pb_tile_at(at.j, pb_tiles(seq(at.b), group));
             const PbTile t = pb_tile(seq(at.b), group, 1.0 / group, ti);
             const uint32_t end = at_end ? stop.k : t.kv;
-            const uint64_t tile_end = line + pb_tile_work(seq(at.b), group, ti);
+            const double tile_end = line + pb_tile_work(seq(at.b), group, ti);
             if (count < max) {
                 const bool begins = at.k == 0 && end < t.kv;
                 const uint32_t row[10] = {w, at.kvh, at.b, ti, at.k, end, t.kv, t.row0, t.rows,

@@ -16,6 +16,7 @@
 //     cut over the workgroups, and the lane offsets of a row group's direct-to-LDS loads.
 #pragma once
 
+#include <math.h>
 #include <stdint.h>
 
 #if defined(__HIPCC__)
@@ -224,13 +225,14 @@ struct PbCut {
 };
 
 DS5_HD uint32_t pb_tiles(PbSeq s, uint32_t group) { return (s.n * group + kPbRows - 1) / kPbRows; }
-DS5_HD uint32_t pb_weight(PbSeq s, uint32_t group) { return s.n * group > kPbNarrow ? 5 : 2; }
-DS5_HD uint64_t pb_tile_work(PbSeq s, uint32_t group, uint32_t tile) {
-    return (uint64_t)group * kPbTileCost + pb_weight(s, group) * ((uint64_t)group * s.before + (uint64_t)kPbRows * (tile + 1));
+// Work as a double that holds an integer below 2^53 (the device multiplies 64-bit integers several times slower).
+DS5_HD double pb_weight(PbSeq s, uint32_t group) { return s.n * group > kPbNarrow ? 5.0 : 2.0; }
+DS5_HD double pb_tile_work(PbSeq s, uint32_t group, uint32_t tile) {
+    return (double)group * kPbTileCost + pb_weight(s, group) * ((double)group * s.before + (double)kPbRows * (tile + 1));
 }
-DS5_HD uint64_t pb_seq_work(PbSeq s, uint32_t group) {
-    const uint64_t nt = pb_tiles(s, group);
-    return nt * group * kPbTileCost + pb_weight(s, group) * (nt * group * s.before + kPbRows / 2 * nt * (nt + 1));
+DS5_HD double pb_seq_work(PbSeq s, uint32_t group) {
+    const double nt = pb_tiles(s, group);
+    return nt * ((double)group * kPbTileCost + pb_weight(s, group) * ((double)group * s.before + kPbRows / 2 * (nt + 1.0)));
 }
 DS5_HD uint32_t pb_tile_at(uint32_t j, uint32_t nt) { return j % 2 ? j / 2 : nt - 1 - j / 2; }
 // x / d with inv = 1.0 / d: the floor of (x + 1/2) / d, which is half of 1 / d or more away from every integer.
@@ -238,12 +240,6 @@ DS5_HD uint32_t pb_over(uint32_t x, double inv) { return (uint32_t)(((double)x +
 DS5_HD PbTile pb_tile(PbSeq s, uint32_t group, double inv_group, uint32_t tile) {
     const uint32_t all = s.n * group, row0 = tile * kPbRows, end = umin(all, row0 + kPbRows);
     return PbTile{row0, end - row0, s.before + pb_over(end - 1, inv_group) + 1};
-}
-// The work before the j-th tile of a sequence's order.
-DS5_HD uint64_t pb_before(PbSeq s, uint32_t group, uint32_t j) {
-    const uint32_t nt = pb_tiles(s, group);
-    const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
-    return j / 2 * pair + (j % 2 ? pb_tile_work(s, group, nt - 1 - j / 2) : 0);
 }
 // 1 / d for d from 1 on, to 2^-44 or better: the device's estimate (to 2^-22) and one step of Newton's method.
 // (A division of doubles takes several times as long there, one of 64-bit integers longer still.)
@@ -255,72 +251,65 @@ DS5_HD double pb_inverse(double d) {
     return 1.0 / d;
 #endif
 }
-// x = q * d + r, with x below 2^53 and q below 2^32: the quotient in f64 is at most one off.
-DS5_HD uint32_t pb_divide(uint64_t x, uint64_t d, uint64_t& r) {
-    uint32_t q = (uint32_t)((double)x * pb_inverse((double)d));
-    int64_t left = (int64_t)(x - (uint64_t)q * d);
-    if (left < 0) {
-        q--;
-        left += (int64_t)d;
-    } else if ((uint64_t)left >= d) {
-        q++;
-        left -= (int64_t)d;
+// x = q * d + r in integers, q below 2^32: the rounded quotient is at most one off.
+DS5_HD uint32_t pb_divide(double x, double d, double& r) {
+    double q = floor(x * pb_inverse(d));
+    r = fma(-q, d, x);
+    if (r < 0.0) {
+        q -= 1.0;
+        r += d;
+    } else if (r >= d) {
+        q += 1.0;
+        r -= d;
     }
-    r = (uint64_t)left;
-    return q;
+    return (uint32_t)q;
 }
-// The cut at y of a sequence's work: tile j of its order (j may be one past the last), position k.
-DS5_HD void pb_locate(PbSeq s, uint32_t group, double inv_group, uint64_t y, uint64_t snap, uint64_t lead, bool whole, uint32_t& j, uint32_t& k) {
+// The cut at y of a sequence's work: tile j of its order (j may be one past the last) that begins
+// `at` into that work, position k.
+struct PbPlace {
+    uint32_t j, k;
+    double at;
+};
+DS5_HD PbPlace pb_locate(PbSeq s, uint32_t group, double inv_group, double y, double snap, double lead, bool whole) {
     const uint32_t nt = pb_tiles(s, group);
-    const uint64_t pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
-    uint64_t off;
-    j = pb_divide(y, pair, off) * 2;
-    const uint64_t heavy = pb_tile_work(s, group, pb_tile_at(j, nt));
+    const double pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
+    double off;
+    uint32_t j = pb_divide(y, pair, off) * 2;
+    const double heavy = pb_tile_work(s, group, pb_tile_at(j, nt));
     if (j + 1 < nt && off >= heavy) {
         j++;
         off -= heavy;
     }
-    k = 0;
     const uint32_t tile = pb_tile_at(j, nt);
-    const uint64_t w = pb_tile_work(s, group, tile);
-    if (whole) {  // cuts between tiles only
-        j += off * 2 >= w;
-        return;
-    }
-    if (off < snap || off <= lead) return;
-    if (w - off < snap) {
-        j++;
-        return;
-    }
+    const double w = pb_tile_work(s, group, tile), at = y - off;
+    if (whole) return off * 2.0 >= w ? PbPlace{j + 1, 0, at + w} : PbPlace{j, 0, at};  // cuts between tiles only
+    if (off < snap || off <= lead) return PbPlace{j, 0, at};
+    if (w - off < snap) return PbPlace{j + 1, 0, at + w};
     const uint32_t kv = pb_tile(s, group, inv_group, tile).kv;
-    k = umin((uint32_t)((double)kv * (double)(off - lead) * pb_inverse((double)(w - lead))), kv - 1) / kPbUnit * kPbUnit;
+    return PbPlace{j, umin((uint32_t)(kv * (off - lead) * pb_inverse(w - lead)), kv - 1) / kPbUnit * kPbUnit, at};
 }
-// The cut before workgroup w of n on a line of `work` (below 2^53): rounded, but never backwards as w
-// grows, and the same wherever it is worked out. part: 1.0 / n.
-DS5_HD uint64_t pb_cut_at(uint64_t work, uint32_t w, uint32_t n, double part) {
-    return w >= n ? work : (uint64_t)((double)work * ((double)w * part));
-}
+// The cut before workgroup w of n on a line of `work`: rounded, but never backwards as w grows, and
+// the same wherever it is worked out. part: 1.0 / n.
+DS5_HD double pb_cut_at(double work, uint32_t w, uint32_t n, double part) { return w >= n ? work : floor(work * (w * part)); }
 // The last workgroup whose cut is at most x (x below work).
-DS5_HD uint32_t pb_last_cut(uint64_t work, uint32_t n, double part, uint64_t x) {
-    uint32_t w = umin((uint32_t)((double)x / (double)work * (double)n), n - 1);
+DS5_HD uint32_t pb_last_cut(double work, uint32_t n, double part, double x) {
+    uint32_t w = umin((uint32_t)(x * pb_inverse(work) * n), n - 1);
     while (w > 0 && pb_cut_at(work, w, n, part) > x) w--;
     while (w + 1 < n && pb_cut_at(work, w + 1, n, part) <= x) w++;
     return w;
 }
-DS5_HD uint64_t pb_snap(uint64_t work, double part, uint32_t group) {
-    const uint64_t share = (uint64_t)((double)work * part * 0.0625), least = (uint64_t)group * (kPbUnit / 2);
-    return share > least ? share : least;
+DS5_HD double pb_snap(double work, double part, uint32_t group) {
+    return fmax(floor(work * part * 0.0625), (double)group * (kPbUnit / 2));
 }
 // A tile's cost that lies before its positions; of tiles that several workgroups share, no more than
 // leaves each of them some.
-DS5_HD uint64_t pb_lead(uint64_t work, double part, uint32_t group) {
-    const uint64_t half = (uint64_t)((double)work * part * 0.5), cost = (uint64_t)group * kPbTileCost;
-    return half < cost ? half : cost;
+DS5_HD double pb_lead(double work, double part, uint32_t group) {
+    return fmin(floor(work * part * 0.5), (double)group * kPbTileCost);
 }
 // The workgroups that share a line of work: kPbPiece of a row's work each at least, and the same number
 // for each kv head where there are enough, so that no workgroup ends one head's tile to begin another's.
-DS5_HD uint32_t pb_workgroups(uint64_t work, uint32_t group, uint32_t heads, uint32_t grid) {
-    const double n = (double)work * pb_inverse((double)group * kPbPiece);
+DS5_HD uint32_t pb_workgroups(double work, uint32_t group, uint32_t heads, uint32_t grid) {
+    const double n = work * pb_inverse((double)group * kPbPiece);
     const uint32_t all = n >= (double)grid ? grid : n < 1.0 ? 1 : (uint32_t)n;
     return all > heads ? all / heads * heads : all;
 }

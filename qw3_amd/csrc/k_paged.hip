@@ -568,7 +568,7 @@ __device__ __noinline__ f32x4 add_odd_values(const f16* vpool, const int32_t* ta
 // is read back by all, so that the loops over positions hold nothing of it in registers.
 struct Walk {
     ds5idx::PbCut at, stop;
-    uint64_t line, total;  // where the tile at `at` begins on the line; the line's length
+    double line, total;  // where the tile at `at` begins on the line; the line's length
     uint32_t wg, n_wg;
     uint32_t more, at_end;           // there is a piece; it is the last
     ds5idx::PbTile tile;
@@ -582,7 +582,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     __shared__ __attribute__((aligned(1024))) char s_kv[A::AREA];
     __shared__ uint32_t s_start[kMaxSeqs], s_n[kMaxSeqs], s_before[kMaxSeqs];
     __shared__ float s_m[kWaves][32], s_l[kWaves][32];
-    __shared__ uint64_t s_scan[kWaves];
+    __shared__ double s_scan[kWaves];
     __shared__ Walk s_walk;
     __shared__ uint32_t s_bad, s_odd, s_broken;
     __shared__ uint32_t s_groups[kWindow];  // of a window of the piece: each 16 positions' group of rows in the pool
@@ -600,7 +600,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         // The workgroup's two halves do the same for the part's two cuts: a thread's sequences are consecutive ones.
         constexpr uint32_t kHalf = kThreads / 2;
         const uint32_t cut = uniform(tid / kHalf), i = tid % kHalf, N = (n_seqs + kHalf - 1) / kHalf, b0 = i * N;
-        uint64_t mine = 0;
+        double mine = 0.0;
 #pragma unroll 1
         for (uint32_t b = b0; b < min(b0 + N, n_seqs); b++) {
             const int64_t s0 = bt.starts[b], s1 = bt.starts[b + 1], len = bt.seq_lens[b];
@@ -612,53 +612,52 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             s_before[b] = ok ? (uint32_t)(len - n) : kPoison;
             mine += ds5idx::pb_seq_work(seq(b), G);
         }
-        uint64_t upto = mine;  // inclusive over the wavefront
+        double upto = mine;  // inclusive over the wavefront
         if (n_seqs > 1) {
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
-                const uint64_t y = __shfl_up(upto, o, 64);
+                const double y = __shfl_up(upto, o, 64);
                 if ((int)lane >= o) upto += y;
             }
         }
-        if (lane == 63 || n_seqs == 1) s_scan[wave] = n_seqs > 1 ? upto : uniform64(mine);
+        if (lane == (n_seqs > 1 ? 63u : 0u)) s_scan[wave] = upto;
         __syncthreads();
-        uint64_t from = upto - mine, per_head = 0;
+        double from = upto - mine, per_head = 0.0;
 #pragma unroll
         for (uint32_t w = 0; w < (uint32_t)kWaves / 2; w++) {
-            const uint64_t x = s_scan[cut * (kWaves / 2) + w];
-            from += w < wave % (kWaves / 2) ? x : 0;
+            const double x = s_scan[cut * (kWaves / 2) + w];
+            from += w < wave % (kWaves / 2) ? x : 0.0;
             per_head += x;
         }
-        per_head = uniform64(per_head);
-        const uint64_t total = per_head * bt.n_kv_heads;
+        const double total = per_head * bt.n_kv_heads;
         const uint32_t grid = gridDim.x;
-        const uint32_t n_wg = total == 0 ? 0 : p.whole ? grid : ds5idx::pb_workgroups(total, G, bt.n_kv_heads, grid);
+        const uint32_t n_wg = uniform(total == 0.0 ? 0 : p.whole ? grid : ds5idx::pb_workgroups(total, G, bt.n_kv_heads, grid));
         // A full grid's consecutive parts go to one XCD (workgroup i runs on XCD i % 8), so that a
         // sequence's K and V come into few L2s.
         const uint32_t wg = n_wg + bt.n_kv_heads > grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
         if (tid == 0 && p.descs) p.descs[wg].rows = 0;  // until it begins a tile that it does not end
         if (wg >= n_wg) return;
-        const double share = 1.0 / (double)n_wg;
-        const uint64_t snap = ds5idx::pb_snap(total, share, G);
+        const double share = ds5idx::pb_inverse(n_wg);
+        const double snap = ds5idx::pb_snap(total, share, G);
         if (tid == 0) {
             s_walk.total = total;
             s_walk.wg = wg, s_walk.n_wg = n_wg;
             s_walk.at_end = 0;
             if (wg + 1 == n_wg) s_walk.stop = ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0};
         }
-        uint64_t y;
+        double y;
         const uint32_t h = ds5idx::pb_divide(ds5idx::pb_cut_at(total, wg + cut, n_wg, share), per_head, y);
         if (y >= from && y - from < mine && wg + cut < n_wg)
             for (uint32_t b = b0;; b++) {
-                const uint64_t work = ds5idx::pb_seq_work(seq(b), G);
+                const double work = ds5idx::pb_seq_work(seq(b), G);
                 if (y - from >= work) {
                     from += work;
                     continue;
                 }
-                uint32_t j, k;
-                ds5idx::pb_locate(seq(b), G, p.inv_group, y - from, snap, ds5idx::pb_lead(total, share, G), p.whole, j, k);
-                (cut ? s_walk.stop : s_walk.at) = ds5idx::PbCut{h, b, j, k};
-                if (cut == 0) s_walk.line = h * per_head + from + ds5idx::pb_before(seq(b), G, j);
+                const ds5idx::PbPlace at =
+                    ds5idx::pb_locate(seq(b), G, p.inv_group, y - from, snap, ds5idx::pb_lead(total, share, G), p.whole);
+                (cut ? s_walk.stop : s_walk.at) = ds5idx::PbCut{h, b, at.j, at.k};
+                if (cut == 0) s_walk.line = h * per_head + from + at.at;
                 break;
             }
     }
@@ -1003,11 +1002,11 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         if (tid == 0) {
             Walk& w = s_walk;
             const ds5idx::PbSeq sq = seq(w.at.b);
-            const uint64_t tile_end =
+            const double tile_end =
                 w.line + ds5idx::pb_tile_work(sq, G, ds5idx::pb_tile_at(w.at.j, ds5idx::pb_tiles(sq, G)));
             // the last workgroup with a part of the tile: the last cut that is not within `snap` of its end
             if (begins && !poison) {
-                const double share = 1.0 / (double)w.n_wg;
+                const double share = ds5idx::pb_inverse(w.n_wg);
                 p.descs[wg] = MergeDesc{ds5idx::pb_last_cut(w.total, w.n_wg, share, tile_end - ds5idx::pb_snap(w.total, share, G)),
                                         rows, row0, kvh, start};
             }
@@ -1139,6 +1138,23 @@ int launch_paged_append(ds5_hip_ctx* ctx, const PagedAppendLaunch& a) {
     return ds5_after_launch(ctx, name);
 }
 
+// Whether uncut tiles are the faster form, in the plan's units (4.7 ns), every sequence taken to have the
+// mean rows and the longest length: rounds of whole tiles, all beginning together (so that their reading at
+// the memory's rate, 23 KB a unit, begins later), or even shares, in which a workgroup pays for a second
+// tile as a rule, and the merge with the parts' way through memory. Measured, us, cut and whole (32 query
+// and 4 kv heads of 128): one token 15.6 and 14.2 at 500 positions, 16.1 and 17.4 at 1000; 48 sequences'
+// 29.1 and 18.3, 33.9 and 24.8, at 2000 42.9 and 51.7; six tokens 19.0 and 22.5, 20.1 and 31.9, 48
+// sequences of six 48.3 and 26.4, 45 and 36.4; eight of 40 31.7 and 25.4, 41.7 and 34.8, 46.6 and 55.5.
+static bool whole_tiles_do(const PagedBatch& b, uint32_t group, uint32_t cus) {
+    const double live = std::min(b.n_seqs, b.n_tokens), rows = std::ceil(b.n_tokens / live) * group;
+    const bool wide = rows > kNarrow;
+    const double tile = ds5idx::kPbTileCost + (wide ? 5.0 : 2.0) * b.max_seq_len, tiles = b.n_kv_heads * live * std::ceil(rows / kRows);
+    const double n = std::min<double>(cus, std::max(1.0, tiles * tile / ds5idx::kPbPiece));
+    const double stream = 4.0 * b.head_dim * b.n_kv_heads * live * b.max_seq_len / 23000.0;
+    const double whole = std::max(std::ceil(tiles / cus) * tile, ds5idx::kPbTileCost + stream);
+    return whole <= tiles / n * tile + ds5idx::kPbTileCost + 1350.0 + (wide ? 1300.0 : 300.0) * n / cus;
+}
+
 int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     const PagedBatch& b = a.batch;
     AttnParams p{};
@@ -1150,12 +1166,10 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     // the work that the plan counts, at most: below 2^53
     if ((double)b.n_kv_heads * tiles * ((double)p.group * (5.0 * b.max_seq_len + ds5idx::kPbTileCost) + 5.0 * (rows + kRows)) >= 9007199254740992.0)
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "paged_attention: batch too large");
-    // Up to 256 positions a workgroup's eight wavefronts take a tile in one go: none is cut then,
-    // and nothing merged. (Nor without the context's memory for parts.)
-    p.whole = !ctx->split_buf || b.max_seq_len <= 256;
+    const uint32_t cus = std::min(kMaxGrid, ctx->cu_count > 0 ? (uint32_t)ctx->cu_count : kMaxGrid);
+    p.whole = !ctx->split_buf || whole_tiles_do(b, p.group, cus);
     const uint64_t most =
         b.n_kv_heads * tiles * (p.whole ? 1 : (5ull * b.max_seq_len + ds5idx::kPbTileCost) / ds5idx::kPbPiece + 1);
-    const uint32_t cus = std::min(kMaxGrid, ctx->cu_count > 0 ? (uint32_t)ctx->cu_count : kMaxGrid);
     const dim3 grid((uint32_t)std::min<uint64_t>(most, cus)), block(kThreads);
     if (!p.whole) {
         static_assert(2ull * kMaxGrid * kRows * 128 * sizeof(float) <= kSplitBytesMax, "parts fit the context's buffer");
