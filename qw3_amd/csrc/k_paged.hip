@@ -375,7 +375,7 @@ struct Attn {
     // Addresses: a block's base plus the lane's offset, then the swizzled chunk by xor (a block begins on a
     // multiple of the row's RB bytes, so that xor in the low bits stays in the row).
     __device__ __forceinline__ static f16x8 kread(uint32_t k, int ks) {
-        return *(const __attribute__((address_space(3))) f16x8*)(k ^ (32 * ks));
+        return *(const __attribute__((address_space(3))) f16x8*)(uintptr_t)(k ^ (32 * ks));
     }
     // positions 16 s + [0, 16): the transpose read gives lane i of 16 column i of 4 rows; element jj of the
     // operand is position 16 s + 8 (jj / 4) + 4 h + jj % 4, as the weights lie
@@ -383,8 +383,8 @@ struct Attn {
         typedef __attribute__((__vector_size__(4 * sizeof(__fp16)))) __fp16 v4h;
         typedef __attribute__((address_space(3))) v4h lds_v4h;
         const uint32_t at = (v ^ (64 * dt)) + 16 * s * RB;
-        const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h*)at));
-        const f16x4 b = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h*)(at + 8 * RB)));
+        const f16x4 a = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h*)(uintptr_t)at));
+        const f16x4 b = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4f16((lds_v4h*)(uintptr_t)(at + 8 * RB)));
         return f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
     __device__ __forceinline__ void product(f32x16& S, const f16x8& k, int ks) const {
