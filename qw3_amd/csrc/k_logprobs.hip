@@ -11,7 +11,10 @@
 // once into registers and used for the maximum, the sums and the selection. Its segment's
 // state: m, S, C, A = sum (x_j - m) e_j, the target's logit where the segment holds it, and
 // the top_n largest keys in order. logprobs_join_kernel: a workgroup per row joins the
-// segments' states. Memory bound: the logits are read once.
+// segments' states. Memory bound: the logits are read once; 512 rows of 65536 (134 MB) with five
+// alternatives take 27 us, 5.0 TB/s, and the join 5. One row of 65536 with 20 alternatives: two
+// launches of 5 us. (The join by the row's last segment, behind a fence and a counter, took longer:
+// 11.2 us instead of 10.2 for one row of 32768, 83 instead of 19 for 600 of 13578.)
 //
 // Selection by unique 64-bit keys (the logit in an order-preserving form above the complement of
 // its index, so that equal logits fall to the lower index): a bound that top_n to 1.5 top_n of the
