@@ -1161,20 +1161,17 @@ int launch_paged_append(ds5_hip_ctx* ctx, const PagedAppendLaunch& a) {
 }
 
 // Whether uncut tiles are the faster form, in the plan's units (4.7 ns), every sequence taken to have the
-// mean rows and the longest length: rounds of whole tiles, all beginning together (so that their reading at
-// the memory's rate, 23 KB a unit, begins later), or even shares, in which a workgroup pays for a second
-// tile as a rule, and the merge with the parts' way through memory. Measured, us, cut and whole (32 query
-// and 4 kv heads of 128): one token 15.6 and 14.2 at 500 positions, 16.1 and 17.4 at 1000; 48 sequences'
-// 29.1 and 18.3, 33.9 and 24.8, at 2000 42.9 and 51.7; six tokens 19.0 and 22.5, 20.1 and 31.9, 48
-// sequences of six 48.3 and 26.4, 45 and 36.4; eight of 40 31.7 and 25.4, 41.7 and 34.8, 46.6 and 55.5.
+// mean rows and the longest length: rounds of whole tiles, or even shares, in which a workgroup pays for a
+// second tile as a rule, and the merge with the parts' way through memory. Measured, us, cut and whole
+// (32 query and 4 kv heads of 128): one token 15.6 and 14.4 at 500 positions, 16.1 and 17.5 at 1000; 48
+// sequences' 29.1 and 18.5, 33.8 and 24.6, at 2000 43.5 and 39.7; six tokens 18.9 and 22.6, 20.3 and 31.7;
+// 48 sequences of six 37.4 and 26.3, 44.5 and 36.1; eight of 40 31.8 and 25.5, 42.0 and 35.1, 47.0 and 55.6.
 static bool whole_tiles_do(const PagedBatch& b, uint32_t group, uint32_t cus) {
     const double live = std::min(b.n_seqs, b.n_tokens), rows = std::ceil(b.n_tokens / live) * group;
     const bool wide = rows > kNarrow;
     const double tile = ds5idx::kPbTileCost + (wide ? 5.0 : 2.0) * b.max_seq_len, tiles = b.n_kv_heads * live * std::ceil(rows / kRows);
     const double n = std::min<double>(cus, std::max(1.0, tiles * tile / ds5idx::kPbPiece));
-    const double stream = 4.0 * b.head_dim * b.n_kv_heads * live * b.max_seq_len / 23000.0;
-    const double whole = std::max(std::ceil(tiles / cus) * tile, ds5idx::kPbTileCost + stream);
-    return whole <= tiles / n * tile + ds5idx::kPbTileCost + 1350.0 + (wide ? 1300.0 : 300.0) * n / cus;
+    return std::ceil(tiles / cus) * tile <= tiles / n * tile + ds5idx::kPbTileCost + 1350.0 + (wide ? 1300.0 : 300.0) * n / cus;
 }
 
 int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
