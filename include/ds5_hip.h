@@ -13,8 +13,8 @@
  *   2. the kernel-provider ops of the attention path, replacing
  *      rmsNorm / rope / kvAppend / gqaAttention of contracts.assertKernelApi
  *      (src/shared/contracts.zig:358-367), plus the matmul of the projections
- *      on either side of it, and fused and paged extensions that the engine
- *      may pick up with @hasDecl.
+ *      on either side of it, fused and paged extensions that the engine
+ *      may pick up with @hasDecl, and the scores of a forward's tokens.
  *
  * Status codes are contracts.KernelError (src/shared/contracts.zig:201-206):
  * every precondition the reference checks is checked here before any launch.
@@ -59,7 +59,7 @@ typedef struct ds5_hip_ctx ds5_hip_ctx;
 
 /* Ctx.init (metal.zig:131, ctx.zig:20): picks device `device_index`
  * (0 for the first visible GPU) and creates the context's stream, timing
- * events and the 32 MiB that attention launches split over their keys use. */
+ * events and the 33 MiB that attention launches split over their keys use. */
 int ds5_hip_init(int device_index, ds5_hip_ctx** out);
 
 /* Ctx.deinit (ctx.zig:26-30): waits for the stream, frees every buffer the
@@ -198,7 +198,7 @@ int ds5_hip_kv_append(ds5_hip_ctx* ctx, const ds5_kv_append_args* args);
  * kernel. All paths are device code. Prefill and f32 launches that would leave
  * compute units idle split their positions and merge the parts: by the shape alone,
  * so a captured call gives the eager call's bits (the parts lie in the context's own
- * 32 MiB, allocated at init; a context without it runs them unsplit). */
+ * 33 MiB, allocated at init; a context without it runs them unsplit). */
 typedef struct ds5_attn_args {
     ds5_buf q;       /* f32 [n_tokens, n_q_heads, head_dim], post-norm post-rope */
     ds5_buf k_cache; /* kv_dtype [n_kv_heads, max_ctx, head_dim] */
@@ -579,7 +579,8 @@ int ds5_hip_paged_append(ds5_hip_ctx* ctx, const ds5_paged_append_args* args);
  * f16 q (as ds5_hip_paged_append writes it) as it is; the softmax weights with 22
  * bits in either case. What a row does not attend never touches it, whatever the
  * pool holds there (infinities and NaN included). At most DS5_PAGED_MAX_SEQS
- * sequences; out must not overlap q or the pools. */
+ * sequences; out must not overlap q or the pools. The same call gives the same
+ * bits every time, captured or not. */
 #define DS5_PAGED_MAX_SEQS 1024u
 typedef struct ds5_paged_attention_args {
     ds5_buf q;          /* q_dtype [n_tokens, n_q_heads, head_dim], normalised and rotated */
