@@ -606,6 +606,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     __shared__ double s_scan[kWaves];
     __shared__ Walk s_walk;
     __shared__ uint32_t s_bad, s_odd, s_broken;
+    __shared__ uint64_t s_row[kRows];  // of the tile's rows: the row of q and of the output (or of the parts)
     __shared__ uint32_t s_groups[kWindow];  // of a window of the piece: each 16 positions' group of rows in the pool
 
     const uint32_t tid = threadIdx.x, lane = tid & 63;
@@ -732,11 +733,9 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             const uint32_t start = uniform(wk.start);
             if constexpr (narrow)
                 A::fetch_q(query, p, ((uint64_t)(start + token) * bt.n_q_heads + kvh * G + (row - token * G)) * D + 8 * h);
-            else {
-                A::stage_q(lds_addr(s_kv) + A::AREA / 2, p.a.q, wave, lane, [&](uint32_t r) -> uint64_t {
-                    const uint32_t packed = row0 + min(r, rows - 1), token = ds5idx::pb_over(packed, p.inv_group);
-                    return (uint64_t)(start + token) * bt.n_q_heads + kvh * G + (packed - token * G);
-                });
+            if (tid < (uint32_t)kRows) {
+                const uint32_t packed = row0 + min(tid, rows - 1), token = ds5idx::pb_over(packed, p.inv_group);
+                s_row[tid] = (uint64_t)(start + token) * bt.n_q_heads + kvh * G + (packed - token * G);
             }
 
             const uint64_t head = (uint64_t)kvh * bt.n_pages * bt.page_size * D;
@@ -820,6 +819,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                 if (work) prime();
             } else {
                 if (work) {
+                    A::stage_q(lds_addr(s_kv) + A::AREA / 2, p.a.q, wave, lane, [&](uint32_t r) { return s_row[r]; });
                     for (uint32_t i = 0; i < 2; i++) {
                         const uint32_t g = uniform(group_at(i));
                         step_k(i, g);
@@ -844,9 +844,9 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) t.O[dt] = f32x16{};
                 bool odd = false;
-                auto clean = [&](char* sv, uint32_t key0) {  // V rows that some row of the tile does not attend
+                auto clean = [&](char* sv, uint32_t key0) {  // what V holds past the end, and infinities and NaN
                     if (key0 + 32 > end) A::zero_tail(sv, key0, end, lane);
-                    if (careful || lim_hi > lim_lo) odd |= A::clean(sv, lane);
+                    if (careful) odd |= A::clean(sv, lane);
                 };
                 for (bool more = work; more;) {
                     if constexpr (narrow) {
@@ -967,52 +967,59 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         const uint32_t slot = 2 * wg + (begins ? 1 : 0);
         const bool any_odd = uniform(s_odd) != 0;
         const uint32_t bad_pos = uniform(s_bad);
+        constexpr uint32_t N = narrow ? kWaves : 2, STEP = kWaves / N;  // wavefronts that hold a part of a row
+        const bool output = done || poison;  // else a part
+        // a row's factors; what a part keeps of it
+        auto factors = [&](uint32_t rr, float (&f)[N], bool keep) {
+            const uint32_t w0 = narrow ? 0 : rr >> 5, r = rr & 31;
+            float M = s_m[w0][r], L = 0.0f;
+#pragma unroll
+            for (uint32_t i = 1; i < N; i++) M = fmaxf(M, s_m[w0 + STEP * i][r]);
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) {
+                const float m = s_m[w0 + STEP * i][r];
+                f[i] = m == -INFINITY ? 0.0f : fast_exp2(m - M);  // (a wavefront that saw none of the row's positions: O is 0)
+                L = __builtin_fmaf(s_l[w0 + STEP * i][r], f[i], L);
+            }
+            if (poison || before + ds5idx::pb_over(row0 + rr, p.inv_group) >= bad_pos) M = 0.0f, L = NAN;
+            if (!output && keep) p.part_ml[(uint64_t)slot * kRows + rr] = float2{M, L};
+            const float unit = output ? 1.0f / L : 1.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) f[i] *= unit;
+        };
+        if constexpr (!narrow) {  // worked out once a row, and kept in place of its references
+            if (tid < rows) {
+                float f[N];
+                factors(tid, f, true);
+                if (!output) s_row[tid] = (uint64_t)slot * kRows + tid;
+#pragma unroll
+                for (uint32_t i = 0; i < N; i++) s_m[(tid >> 5) + STEP * i][tid & 31] = f[i];
+            }
+            __syncthreads();
+        }
         {
             // a row's D / 4 columns to as many threads, kThreads / CH rows at a time
-            constexpr uint32_t CH = A::CH, PER = kThreads / CH;
+            constexpr uint32_t CH = A::CH, PER = kThreads / CH, U = narrow ? 1 : 4;
             const uint32_t c = here(tid) % CH, stride = narrow ? 2 * HALF : 8 * HALF;
-            auto fold = [&](uint32_t r, uint32_t w0, float& M, float& L, f32x4& o, auto parts) {
-                constexpr uint32_t N = decltype(parts)::value, STEP = kWaves / N;
-                float mw[N], f[N];
-                f32x4 v[N];
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++) {
-                    mw[i] = s_m[w0 + STEP * i][r];
-                    v[i] = *(const f32x4*)(s_kv + w0 * 2 * HALF + i * stride + r * 4 * D + (c ^ (r & (CH - 1))) * 16);
-                }
-                M = mw[0];
-#pragma unroll
-                for (uint32_t i = 1; i < N; i++) M = fmaxf(M, mw[i]);
-                L = 0.0f, o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (uint32_t i = 0; i < N; i++) {
-                    f[i] = mw[i] == -INFINITY ? 0.0f : fast_exp2(mw[i] - M);  // (a wavefront that saw none of the row's positions: O is 0)
-                    L = __builtin_fmaf(s_l[w0 + STEP * i][r], f[i], L);
-                    o += v[i] * f[i];
-                }
-            };
+            float* const to = output ? p.a.out : p.part_o;
             auto finish = [&](uint32_t rr) {
-                float M, L;
-                f32x4 o;
-                if constexpr (narrow) fold(rr, 0, M, L, o, std::integral_constant<uint32_t, kWaves>{});
-                else fold(rr & 31, rr >> 5, M, L, o, std::integral_constant<uint32_t, 2>{});
-                const uint32_t packed = row0 + rr, token = ds5idx::pb_over(packed, p.inv_group), pos = before + token;
+                const uint32_t w0 = narrow ? 0 : rr >> 5, r = rr & 31;
+                float f[N];
+                if constexpr (narrow) factors(rr, f, c == 0);
+                else
+                    for (uint32_t i = 0; i < N; i++) f[i] = s_m[w0 + STEP * i][r];
+                f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (uint32_t i = 0; i < N; i++)
+                    o += *(const f32x4*)(s_kv + w0 * 2 * HALF + i * stride + r * 4 * D + (c ^ (r & (CH - 1))) * 16) * f[i];
                 if (any_odd) {
                     const PagedBatch& bt = p.a.batch;
                     o = add_odd_values(p.a.v_pool + (uint64_t)kvh * bt.n_pages * bt.page_size * D,
                                        bt.page_table + (uint64_t)wk.at.b * bt.max_pages, bt.page_size, bt.n_pages, D, kb,
-                                       min(end, pos + 1), c, o);
+                                       min(end, before + ds5idx::pb_over(row0 + rr, p.inv_group) + 1), c, o);
                 }
-                if (poison || pos >= bad_pos) M = 0.0f, L = NAN;
-                if (done || poison) {
-                    const uint64_t to = ((uint64_t)(start + token) * p.a.batch.n_q_heads + kvh * G + (packed - token * G)) * D + 4 * c;
-                    *(f32x4*)(p.a.out + to) = o * (1.0f / L);
-                } else {
-                    *(f32x4*)(p.part_o + ((uint64_t)slot * kRows + rr) * D + 4 * c) = o;
-                    if (c == 0) p.part_ml[(uint64_t)slot * kRows + rr] = float2{M, L};
-                }
+                *(f32x4*)(to + (narrow && !output ? (uint64_t)slot * kRows + rr : s_row[rr]) * D + 4 * c) = o;
             };
-            constexpr uint32_t U = narrow ? 1 : 4;  // rows at a time, for their reads from LDS to wait together
 #pragma unroll 1
             for (uint32_t r = here(tid) / CH; r < rows; r += U * PER)
 #pragma unroll
