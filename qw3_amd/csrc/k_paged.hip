@@ -643,6 +643,10 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             }
         }
         if (lane == (n_seqs > 1 ? 63u : 0u)) s_scan[wave] = upto;
+        if (tid == 0) {  // where decreasing starts make more work than the sums hold exactly: no part
+            s_walk.at = s_walk.stop = ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0};
+            s_walk.line = 0.0;
+        }
         __syncthreads();
         double from = upto - mine, per_head = 0.0;
 #pragma unroll
@@ -665,12 +669,11 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             s_walk.total = total;
             s_walk.wg = wg, s_walk.n_wg = n_wg;
             s_walk.at_end = 0;
-            if (wg + 1 == n_wg) s_walk.stop = ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0};
         }
         double y;
         const uint32_t h = ds5idx::pb_divide(ds5idx::pb_cut_at(total, wg + cut, n_wg, share), per_head, y);
         if (y >= from && y - from < mine && wg + cut < n_wg)
-            for (uint32_t b = b0;; b++) {
+            for (uint32_t b = b0; b < min(b0 + N, n_seqs); b++) {
                 const double work = ds5idx::pb_seq_work(seq(b), G);
                 if (y - from >= work) {
                     from += work;

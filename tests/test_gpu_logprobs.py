@@ -253,3 +253,41 @@ def test_nan_alone_in_a_segment(ctx, hip, V, at, rest):
     lp, ent, ids, tops = run(ctx, hip, x, np.zeros(2, int), 3)
     assert np.isfinite([lp[0], ent[0], *tops[0]]).all()
     assert np.isnan([lp[1], ent[1], *tops[1]]).all() and np.all(ids[1] == -1)
+
+
+def test_two_graphs_share_the_workspaces(ctx, hip):
+    """Attention and scores of two shapes, each in a graph of its own, replayed in turn with eager calls that outgrow
+    the workspace between them: every replay as the eager calls, bit for bit."""
+    from batches import Batch
+    calls = []
+    for seed, lens, new, n, V in ((1, [5000, 900], [1, 70], 40, 70001), (2, [12000], [1], 3, 300000)):
+        c = Batch(seed, lens, new, 16, 2, 128)
+        out, bufs = ctx.createBuffer(c.rows * c.hq * c.d * 4), [dev(ctx, a) for a in (c.q, c.kp, c.vp, c.table, c.starts, c.seq_lens)]
+        at = hip.PagedAttentionArgs(*bufs, out, *c.shape(hip, False), c.scale)
+        x = dev(ctx, c.g.standard_normal((n, V)).astype(np.float32))
+        outs = [ctx.createBuffer(n * 4) for _ in range(2)] + [ctx.createBuffer(n * 20 * 4) for _ in range(2)]
+        lp = hip.TokenLogprobsArgs(x, dev(ctx, c.g.integers(0, V, n).astype(np.int32)), *outs, n, V, V, 20)
+
+        def both(at=at, lp=lp):
+            hip.pagedAttention(ctx, at)
+            hip.tokenLogprobs(ctx, lp)
+
+        both()
+        got = [ctx.to_numpy(o, np.uint32) for o in (out, *outs)]
+        calls.append((both, ctx.capture(both), (out, *outs), got))
+    big = ctx.createBuffer(8000 * 20000 * 4)  # 6.6 MB of states and keys, more than a workspace begins with
+    ctx.zero(big, big.len)
+    tops = [ctx.createBuffer(8000 * 32 * 4) for _ in range(2)]
+    none = hip.Buf()
+    for i in range(4):
+        for both, graph, outs, want in calls:
+            for o in outs:
+                ctx.zero(o, o.len)
+            graph.launch()
+            assert all(np.array_equal(ctx.to_numpy(o, np.uint32), w) for o, w in zip(outs, want))
+            if i == 1:
+                hip.tokenLogprobs(ctx, hip.TokenLogprobsArgs(big, none, none, none, *tops, 8000, 20000, 20000, 32))
+                assert np.array_equal(ctx.to_numpy(tops[0], np.int32), np.tile(np.arange(32), 8000))
+                both()
+    for _, graph, _, _ in calls:
+        graph.destroy()
