@@ -207,7 +207,7 @@ DS5_HD uint32_t af_row_splits(uint32_t lim, uint32_t chunk) { return lim / chunk
 // Work is counted in half positions * group for the tiles of sequences of at most kPbNarrow rows
 // and in fifths for the others (64 positions measured 0.5 .. 0.7 us and 1.3 .. 1.5), a tile's being
 // its positions (taken as if every tile were full) and before them kPbTileCost for beginning and
-// ending it (10 us and 12). A workgroup whose part begins inside a tile, or ends there, pays that
+// ending it (10 us and 11). A workgroup whose part begins inside a tile, or ends there, pays that
 // as every other does; what counts is the tiles that it begins after another, so the cost lies at
 // the tile's start, and cuts there fall on the start. A cut further on falls on a multiple of
 // kPbUnit positions, or on the tile's start or end where that is no further than `snap`.

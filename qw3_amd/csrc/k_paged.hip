@@ -164,11 +164,11 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppen
 // are folded through LDS at the end. K and V come by direct-to-LDS loads, a block or three steps ahead.
 //
 // What bounds it. Long decode: memory; 32 sequences of 0.5 .. 16 K positions (4 kv heads of 128, 584 MB)
-// 115 us, 5.1 TB/s. Prompts: the matrix cores at the power that they may draw; 64 positions of 128 rows
+// 114 us, 5.1 TB/s. Prompts: the matrix cores at the power that they may draw; 64 positions of 128 rows
 // take 1.3 us with f16 q (48 products of 32 cycles a wavefront pair) and 1.5 with f32 q (64): 1.2 and 1.4
 // PFLOP/s issued, above a large library product's 1.14; leaving out the exponentials, the V reads or the
-// barriers changed neither. A prompt of 2048 71 us, 203 f32 tokens at 6000 88 + 8 merging. Small calls:
-// the chain of launch, plan, page table, K, V and output, 12 .. 15 us and 4 for the merge.
+// barriers changed neither. A prompt of 2048 69 us, 203 f32 tokens at 6000 88 + 8 merging. Small calls:
+// the chain of launch, plan, page table, K, V and output, 9 .. 14 us and 4 for the merge.
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 512, kWaves = 8;
 constexpr int kRows = ds5idx::kPbRows, kNarrow = ds5idx::kPbNarrow;
