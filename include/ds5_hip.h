@@ -543,7 +543,7 @@ int ds5_hip_paged_decode(ds5_hip_ctx* ctx, const ds5_paged_decode_args* args);
  * alone). q_out may be q itself when q_dtype is f32; other overlaps of the
  * outputs with the inputs are ShapeMismatch. A row that shows as NaN (see above)
  * does so in q_out, and its k and v are not appended. Two rows of one call must
- * not share a slot. */
+ * not share a slot. At most 2^24 - 1 rows. */
 typedef struct ds5_paged_append_args {
     ds5_buf q;          /* optional f32 [n_tokens, n_q_heads, head_dim] */
     ds5_buf k;          /* f32 [n_tokens, n_kv_heads, head_dim] */
@@ -621,8 +621,8 @@ int ds5_hip_paged_attention(ds5_hip_ctx* ctx, const ds5_paged_attention_args* ar
  * in f32 relative to the row's maximum, which itself stays out of them, so that
  * the log probability and the entropy of a row that is almost certain keep their
  * relative accuracy. vocab is at most DS5_LOGPROBS_MAX_VOCAB, top_n at most
- * DS5_LOGPROBS_MAX_TOP and at most vocab; views 4-byte aligned, no output
- * overlapping logits. Uses the context workspace: run a shape once before
+ * DS5_LOGPROBS_MAX_TOP and at most vocab, n_rows * ceil(vocab / 8192) below 2^24;
+ * views 4-byte aligned, no output overlapping logits. Uses the context workspace: run a shape once before
  * capturing it in a graph. */
 #define DS5_LOGPROBS_MAX_VOCAB (1u << 21)
 #define DS5_LOGPROBS_MAX_TOP 32u

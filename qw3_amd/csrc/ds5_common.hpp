@@ -468,6 +468,7 @@ struct PagedAttentionLaunch {
 int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a);
 
 // Log probabilities, entropy and top alternatives of rows of logits (k_logprobs.hip).
+constexpr uint32_t kLogprobsSegment = 8192;  // of a row's logits, where the rows fill the device
 struct LogprobsLaunch {
     const float* logits;
     const int32_t* targets;

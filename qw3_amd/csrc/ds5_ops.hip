@@ -1058,6 +1058,9 @@ int ds5_hip_paged_decode(ds5_hip_ctx* ctx, const ds5_paged_decode_args* a) {
     return launch_decode(ctx, l);
 }
 
+// The most workgroups of 256 threads that a launch takes (2^32 - 1 threads along x).
+static constexpr uint32_t kMaxGroups = UINT32_MAX / 256;
+
 // Preconditions of a ragged batch over the paged pool, and the batch.
 static int check_paged_batch(ds5_hip_ctx* ctx, const char* op, const PagedBatch& p, ds5_buf k_pool, ds5_buf v_pool,
                              ds5_buf page_table, ds5_buf starts, ds5_buf seq_lens, uint32_t q_dtype) {
@@ -1108,6 +1111,7 @@ int ds5_hip_paged_append(ds5_hip_ctx* ctx, const ds5_paged_append_args* a) {
     if (!aligned16(a->k) || !aligned16(a->v) || (a->q_norm.len && !aligned16(a->q_norm)) ||
         (a->k_norm.len && !aligned16(a->k_norm)) || (with_q && (!aligned16(a->q) || !aligned16(a->q_out))))
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: views must be 16-byte aligned", op);
+    if (T > kMaxGroups) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: more than %u rows", op, kMaxGroups);
     if (T == 0 || a->n_seqs == 0) return DS5_OK;
     // what is written must not be read as something else by another workgroup
     struct View {
@@ -1192,7 +1196,7 @@ int ds5_hip_token_logprobs(ds5_hip_ctx* ctx, const ds5_token_logprobs_args* a) {
     if (a->row_stride < V) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: row_stride below vocab", op);
     if (top > DS5_LOGPROBS_MAX_TOP || top > V)
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: top_n %u (at most %u and vocab)", op, a->top_n, DS5_LOGPROBS_MAX_TOP);
-    if (n > INT32_MAX || n * a->row_stride > (1ull << 61)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: too many rows", op);
+    if (n * ((V + kLogprobsSegment - 1) / kLogprobsSegment) > kMaxGroups) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: too many rows", op);
     const uint64_t logit_bytes = n ? ((n - 1) * a->row_stride + V) * 4 : 0;
     if (!covers(a->logits, logit_bytes)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: logits too small", op);
     if (a->logprobs.len && !covers(a->targets, n * 4)) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: targets too small", op);

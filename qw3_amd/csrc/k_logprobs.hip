@@ -286,15 +286,14 @@ int launch_token_logprobs(ds5_hip_ctx* ctx, const LogprobsLaunch& a) {
     // one row of 32768 logits with 20 alternatives takes 10.2 us so, 2032 rows of 820 11.4 (17.2 in the longer).
     // A row that fits one segment needs no join: of 8192 logits 7.8 us, in four segments 10.4.
     uint32_t per = 32;
-    uint64_t segs = (a.vocab + 8191) / 8192;
+    uint64_t segs = (a.vocab + kLogprobsSegment - 1) / kLogprobsSegment;
     if (((segs > 1 && segs * a.n_rows < 256) || a.vocab <= 2048) && (a.vocab + 2047) / 2048 <= kMaxSegs) {
         per = 8;
         segs = (a.vocab + 2047) / 2048;
     }
-    static_assert((DS5_LOGPROBS_MAX_VOCAB + 8191) / 8192 <= kMaxSegs, "a join thread per segment");
+    static_assert(32 * kThreads == kLogprobsSegment && DS5_LOGPROBS_MAX_VOCAB / kLogprobsSegment <= kMaxSegs, "a join thread per segment");
     LogprobsParams p{a.logits, a.targets, a.logprobs, a.entropy, a.top_ids, a.top_logprobs, a.vocab, a.row_stride, a.top_n,
                      (uint32_t)segs, nullptr, nullptr};
-    if (segs * a.n_rows > INT32_MAX) return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "token_logprobs: too many rows");
     if (segs > 1) {
         const size_t key_bytes = (size_t)a.n_rows * segs * a.top_n * sizeof(uint64_t);
         void* ws = nullptr;

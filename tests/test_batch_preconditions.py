@@ -137,6 +137,17 @@ def test_logprobs_refusals(hip):
         assert rc_of(hip, fn, logprobs(hip, **{out: hip.Buf(getattr(a, other).handle, 0, getattr(a, out).len)})) == 1, (out, other)
 
 
+def test_more_rows_than_a_launch_takes(hip):
+    """2^24 - 1 workgroups of 256 threads at most, whatever the views hold."""
+    at = {n: hip.Buf((i + 1) << 44, 0, 1 << 43) for i, n in enumerate(("q", "k", "v", "q_norm", "k_norm", "q_out", "k_pool", "v_pool",
+                                                                       "page_table", "starts", "seq_lens"))}
+    for n, rc in ((2 ** 24 - 1, 3), (2 ** 24, 1)):
+        assert rc_of(hip, "ds5_hip_paged_append", append(hip, **at, n_tokens=n)) == rc
+    at = {n: hip.Buf((i + 1) << 44, 0, 1 << 43) for i, n in enumerate(("logits", "targets", "logprobs", "entropy", "top_ids", "top_logprobs"))}
+    for n, V, rc in ((2 ** 24 - 1, 8192, 3), (2 ** 24, 100, 1), (2 ** 23 - 1, 8193, 3), (2 ** 23, 8193, 1), (2 ** 32 - 1, 1, 1)):
+        assert rc_of(hip, "ds5_hip_token_logprobs", logprobs(hip, **at, n_rows=n, vocab=V, row_stride=V, top_n=0)) == rc, (n, V)
+
+
 def test_structs_match_c(hip, tmp_path):
     import subprocess
     import test_abi
