@@ -933,6 +933,23 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
 #pragma unroll
                     for (int e = 0; e < 16; e++) zero[e % 4] = __builtin_fmaf(t.O[dt][e], 0.0f, zero[e % 4]);
                 if (__ballot(!((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f)) != 0 && lane == 0) s_broken = 1;
+                {  // rows of O through LDS
+                    const float l = swap32_op(t.l, OpAdd{});
+                    const uint32_t lane = here(tid) & 63, r32 = lane & 31, h = lane >> 5;
+                    char* area = s_kv + wave * 2 * HALF;
+#pragma unroll
+                    for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t c = 8 * dt + 2 * i + h;
+                            *(float4*)(area + r32 * 4 * D + (c ^ (r32 & (A::CH - 1))) * 16) =
+                                float4{t.O[dt][4 * i], t.O[dt][4 * i + 1], t.O[dt][4 * i + 2], t.O[dt][4 * i + 3]};
+                        }
+                    if (h == 0) {
+                        s_m[wave][r32] = t.m;
+                        s_l[wave][r32] = l;
+                    }
+                }
                 __syncthreads();
                 if (careful || uniform(s_broken) == 0) break;
                 careful = true;
@@ -943,25 +960,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             }
         }
 
-        // ---- the wavefronts' parts of the tile together: rows of O through LDS
-        const float l = swap32_op(t.l, OpAdd{});
-        {
-            const uint32_t lane = here(tid) & 63, r32 = lane & 31, h = lane >> 5;
-            char* area = s_kv + wave * 2 * HALF;
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t c = 8 * dt + 2 * i + h;
-                    *(float4*)(area + r32 * 4 * D + (c ^ (r32 & (A::CH - 1))) * 16) =
-                        float4{t.O[dt][4 * i], t.O[dt][4 * i + 1], t.O[dt][4 * i + 2], t.O[dt][4 * i + 3]};
-                }
-            if (h == 0) {
-                s_m[wave][r32] = t.m;
-                s_l[wave][r32] = l;
-            }
-        }
-        __syncthreads();
+        // ---- the wavefronts' parts of the tile together
         const uint32_t kb = uniform(wk.begin), end = uniform(wk.end), wg = uniform(wk.wg), G = p.group;
         const uint32_t row0 = uniform(wk.tile.row0), rows = uniform(wk.tile.rows), before = uniform(wk.before);
         const uint32_t start = uniform(wk.start), kvh = uniform(wk.at.kvh);
