@@ -585,15 +585,16 @@ __device__ __noinline__ f32x4 add_odd_values(const f16* vpool, const int32_t* ta
     return o;
 }
 
-// The workgroup's way along the batch's line of work, kept in LDS by thread 0; the piece it is at
-// is read back by all, so that the loops over positions hold nothing of it in registers.
+// The workgroup's way along the batch's line of work: its part's cuts; where the tile at hand begins on
+// the line; and what the end of the piece at hand needs of it, read back from LDS so that the loops over
+// positions hold nothing of it in registers.
 struct Walk {
     ds5idx::PbCut at, stop;
-    double line, total;  // where the tile at `at` begins on the line; the line's length
+    double line, total;  // (the line's length)
     uint32_t wg, n_wg;
-    uint32_t more, at_end;           // there is a piece; it is the last
+    ds5idx::PbCut now;
     ds5idx::PbTile tile;
-    uint32_t start, before, poison, begin, end;  // the sequence's first row, tokens before its rows; the piece's positions
+    uint32_t start, before, poison, end;  // the sequence's first row, tokens before its rows; the piece's end
 };
 
 template <int D, bool Q16>
@@ -605,7 +606,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     __shared__ float s_m[kWaves][32], s_l[kWaves][32];
     __shared__ double s_scan[kWaves];
     __shared__ Walk s_walk;
-    __shared__ uint32_t s_bad, s_odd, s_broken;
+    // the first position with a page out of range, infinities or NaN set aside, and met: of the pieces in turn
+    __shared__ uint32_t s_bad[2], s_odd[2], s_broken[2];
     __shared__ uint64_t s_row[kRows];  // of the tile's rows: the row of q and of the output (or of the parts)
     __shared__ uint32_t s_groups[kWindow];  // of a window of the piece: each 16 positions' group of rows in the pool
 
@@ -646,6 +648,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         if (tid == 0) {  // where decreasing starts make more work than the sums hold exactly: no part
             s_walk.at = s_walk.stop = ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0};
             s_walk.line = 0.0;
+            s_bad[0] = 0xffffffffu, s_odd[0] = s_broken[0] = 0;
         }
         __syncthreads();
         double from = upto - mine, per_head = 0.0;
@@ -668,7 +671,6 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         if (tid == 0) {
             s_walk.total = total;
             s_walk.wg = wg, s_walk.n_wg = n_wg;
-            s_walk.at_end = 0;
         }
         double y;
         const uint32_t h = ds5idx::pb_divide(ds5idx::pb_cut_at(total, wg + cut, n_wg, share), per_head, y);
@@ -688,27 +690,27 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
     }
     __syncthreads();
 
-    for (bool last_piece = false; !last_piece;) {
+    auto scalar = [](const ds5idx::PbCut& c) { return ds5idx::PbCut{uniform(c.kvh), uniform(c.b), uniform(c.j), uniform(c.k)}; };
+    ds5idx::PbCut at = scalar(s_walk.at);
+    uint32_t turn = 0;
+    for (bool last_piece = false; !last_piece; at.j++, at.k = 0, turn ^= 1) {
+        // every wavefront walks by itself; what the piece's end needs of it lies in LDS until then
+        const ds5idx::PbCut stop = scalar(s_walk.stop);
+        if (!ds5idx::pb_next(at, stop, n_seqs, p.a.batch.n_kv_heads, p.group,
+                             [&](uint32_t b) { return ds5idx::PbSeq{uniform(s_n[b]), 0}; }, last_piece))
+            return;
+        const Walk& wk = *(const Walk*)((const char*)&s_walk + here(0));
+        const uint32_t mark = uniform(s_before[at.b]), start = uniform(s_start[at.b]);
+        const ds5idx::PbSeq sq{uniform(s_n[at.b]), mark & ~kPoison};
+        ds5idx::PbTile tile = ds5idx::pb_tile(sq, p.group, p.inv_group, ds5idx::pb_tile_at(at.j, ds5idx::pb_tiles(sq, p.group)));
+        tile.kv = uniform(tile.kv);
+        const uint32_t end = last_piece ? stop.k : tile.kv;
         if (tid == 0) {
             Walk& w = s_walk;
-            bool at_end = false;
-            w.more = ds5idx::pb_next(w.at, w.stop, n_seqs, p.a.batch.n_kv_heads, p.group, seq, at_end);
-            if (w.more) {
-                const ds5idx::PbSeq sq = seq(w.at.b);
-                w.tile = ds5idx::pb_tile(sq, p.group, p.inv_group, ds5idx::pb_tile_at(w.at.j, ds5idx::pb_tiles(sq, p.group)));
-                w.start = s_start[w.at.b];
-                w.before = sq.before;
-                w.poison = s_before[w.at.b] & kPoison;
-                w.begin = w.at.k;
-                w.end = at_end ? w.stop.k : w.tile.kv;
-                w.at_end = at_end;
-            }
-            s_bad = 0xffffffffu, s_odd = s_broken = 0;
+            w.now = at;
+            w.tile = tile;
+            w.start = start, w.before = sq.before, w.poison = mark & kPoison, w.end = end;
         }
-        __syncthreads();
-        const Walk& wk = *(const Walk*)((const char*)&s_walk + here(0));
-        if (uniform(wk.more) == 0) return;
-        last_piece = uniform(wk.at_end) != 0;
         // The piece, in a form of its own for tiles of at most kNarrow rows (in one form of both the compiler
         // spills: the accumulators then meet where the forms part and join).
         auto piece = [&](auto form) {
@@ -720,10 +722,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         t.voff = ds5idx::pb_load_off(D, true, 0, lane);
         {
             const typename A::Lane ln(lane);
-            const uint32_t kb = uniform(wk.begin), end = uniform(wk.end);
-            const uint32_t rows = uniform(wk.tile.rows), row0 = uniform(wk.tile.row0), before = uniform(wk.before);
-            const uint32_t kvh = uniform(wk.at.kvh), b = uniform(wk.at.b), G = p.group;
-            const bool poison = uniform(wk.poison) != 0;
+            const uint32_t kb = at.k, rows = tile.rows, row0 = tile.row0, before = sq.before, kvh = at.kvh, b = at.b, G = p.group;
+            const bool poison = (mark & kPoison) != 0;
             const uint32_t rg = narrow ? 0 : wave & 3;
             const PagedBatch& bt = p.a.batch;
             // ---- this wavefront's 32 query rows
@@ -733,7 +733,6 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             const uint32_t lim_lo = uniform(before + ds5idx::pb_over(row0 + min(32 * rg, rows - 1), p.inv_group));
             const uint32_t lim_hi = uniform(before + ds5idx::pb_over(row0 + min(32 * rg + 31, rows - 1), p.inv_group));
             typename A::Query query;
-            const uint32_t start = uniform(wk.start);
             if constexpr (narrow)
                 A::fetch_q(query, p, ((uint64_t)(start + token) * bt.n_q_heads + kvh * G + (row - token * G)) * D + 8 * h);
             if (tid < (uint32_t)kRows) {
@@ -758,7 +757,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                     const uint32_t pos = from + 16 * i, page = ds5idx::pb_over(pos, p.inv_page);
                     const uint32_t pg = (uint32_t)table[page];  // (a page out of range: page 0, and the rows that attend it are NaN)
                     s_groups[i] = (pg < bt.n_pages ? pg : 0) * (page_size / 16) + (pos - page * page_size) / 16;
-                    if (pg >= bt.n_pages) atomicMin(&s_bad, pos);
+                    if (pg >= bt.n_pages) atomicMin(&s_bad[turn], pos);
                 }
                 __syncthreads();
             };
@@ -926,13 +925,13 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                         prime();
                     }
                 }
-                if (odd && lane == 0) s_odd = 1;
+                if (odd && lane == 0) s_odd[turn] = 1;
                 float zero[4] = {};  // (NaN where O holds an infinity or NaN)
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) zero[e % 4] = __builtin_fmaf(t.O[dt][e], 0.0f, zero[e % 4]);
-                if (__ballot(!((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f)) != 0 && lane == 0) s_broken = 1;
+                if (__ballot(!((zero[0] + zero[1]) + (zero[2] + zero[3]) == 0.0f)) != 0 && lane == 0) s_broken[turn] = 1;
                 {  // rows of O through LDS
                     const float l = swap32_op(t.l, OpAdd{});
                     const uint32_t lane = here(tid) & 63, r32 = lane & 31, h = lane >> 5;
@@ -951,7 +950,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                     }
                 }
                 __syncthreads();
-                if (careful || uniform(s_broken) == 0) break;
+                if (careful || uniform(s_broken[turn]) == 0) break;
                 careful = true;
                 if (work) {
                     window(kb);
@@ -961,14 +960,15 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         }
 
         // ---- the wavefronts' parts of the tile together
-        const uint32_t kb = uniform(wk.begin), end = uniform(wk.end), wg = uniform(wk.wg), G = p.group;
+        const uint32_t kb = uniform(wk.now.k), end = uniform(wk.end), wg = uniform(wk.wg), G = p.group;
         const uint32_t row0 = uniform(wk.tile.row0), rows = uniform(wk.tile.rows), before = uniform(wk.before);
-        const uint32_t start = uniform(wk.start), kvh = uniform(wk.at.kvh);
+        const uint32_t start = uniform(wk.start), kvh = uniform(wk.now.kvh);
         const bool done = kb == 0 && end == uniform(wk.tile.kv), poison = uniform(wk.poison) != 0;
         const bool begins = kb == 0 && !done;
         const uint32_t slot = 2 * wg + (begins ? 1 : 0);
-        const bool any_odd = uniform(s_odd) != 0;
-        const uint32_t bad_pos = uniform(s_bad);
+        const bool any_odd = uniform(s_odd[turn]) != 0;
+        const uint32_t bad_pos = uniform(s_bad[turn]);
+        if (tid == 0) s_bad[turn ^ 1] = 0xffffffffu, s_odd[turn ^ 1] = s_broken[turn ^ 1] = 0;  // the next piece's
         constexpr uint32_t N = narrow ? kWaves : 2, STEP = kWaves / N;  // wavefronts that hold a part of a row
         const bool output = done || poison;  // else a part
         // a row's factors; what a part keeps of it
@@ -1017,7 +1017,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                 if (any_odd) {
                     const PagedBatch& bt = p.a.batch;
                     o = add_odd_values(p.a.v_pool + (uint64_t)kvh * bt.n_pages * bt.page_size * D,
-                                       bt.page_table + (uint64_t)wk.at.b * bt.max_pages, bt.page_size, bt.n_pages, D, kb,
+                                       bt.page_table + (uint64_t)wk.now.b * bt.max_pages, bt.page_size, bt.n_pages, D, kb,
                                        min(end, before + ds5idx::pb_over(row0 + rr, p.inv_group) + 1), c, o);
                 }
                 *(f32x4*)(to + (narrow && !output ? (uint64_t)slot * kRows + rr : s_row[rr]) * D + 4 * c) = o;
@@ -1031,9 +1031,9 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         __syncthreads();  // LDS is free again
         if (tid == 0) {
             Walk& w = s_walk;
-            const ds5idx::PbSeq sq = seq(w.at.b);
+            const ds5idx::PbSeq sq = seq(w.now.b);
             const double tile_end =
-                w.line + ds5idx::pb_tile_work(sq, G, ds5idx::pb_tile_at(w.at.j, ds5idx::pb_tiles(sq, G)));
+                w.line + ds5idx::pb_tile_work(sq, G, ds5idx::pb_tile_at(w.now.j, ds5idx::pb_tiles(sq, G)));
             // the last workgroup with a part of the tile: the last cut that is not within `snap` of its end
             if (begins && !poison) {
                 const double share = ds5idx::pb_inverse(w.n_wg);
@@ -1041,11 +1041,9 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                                         rows, row0, kvh, start};
             }
             w.line = tile_end;
-            w.at.j++;
-            w.at.k = 0;
         }
         };
-        if (uniform(wk.tile.rows) <= (uint32_t)kNarrow) piece(std::true_type{});
+        if (tile.rows <= (uint32_t)kNarrow) piece(std::true_type{});
         else piece(std::false_type{});
     }
 }
