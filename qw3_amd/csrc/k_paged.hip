@@ -213,6 +213,28 @@ __device__ __forceinline__ uint64_t uniform64(uint64_t v) {
     return ((uint64_t)uniform((uint32_t)(v >> 32)) << 32) | uniform((uint32_t)v);
 }
 
+// Sums over the wavefront's lanes up to and with this one, in six DPP adds (rows of 16 lanes by shifts of 1, 2, 4
+// and 8, then lane 15 of a row to the next row and lane 31 to the upper half; a lane without a source adds 0).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or_0(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_or_0(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)dpp_or_0<CTRL, ROWS>((uint32_t)(u >> 32)) << 32 | dpp_or_0<CTRL, ROWS>((uint32_t)u));
+}
+template <class T>
+__device__ __forceinline__ T sums_upto(T v) {
+    v += dpp_or_0<0x111, 0xF>(v);
+    v += dpp_or_0<0x112, 0xF>(v);
+    v += dpp_or_0<0x114, 0xF>(v);
+    v += dpp_or_0<0x118, 0xF>(v);
+    v += dpp_or_0<0x142, 0xA>(v);
+    v += dpp_or_0<0x143, 0xC>(v);
+    return v;
+}
+
 template <int N>
 __device__ __forceinline__ void wait_loads() {  // at most N vector-memory operations of the wavefront in flight
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -636,15 +658,8 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             s_before[b] = ok ? (uint32_t)(len - n) : kPoison;
             mine += ds5idx::pb_seq_work(seq(b), G);
         }
-        double upto = mine;  // inclusive over the wavefront
-        if (n_seqs > 1) {
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(upto, o, 64);
-                if ((int)lane >= o) upto += y;
-            }
-        }
-        if (lane == (n_seqs > 1 ? 63u : 0u)) s_scan[wave] = upto;
+        const double upto = sums_upto(mine);
+        if (lane == 63) s_scan[wave] = upto;
         if (tid == 0) {  // where decreasing starts make more work than the sums hold exactly: no part
             s_walk.at = s_walk.stop = ds5idx::PbCut{bt.n_kv_heads, 0, 0, 0};
             s_walk.line = 0.0;
@@ -1065,12 +1080,7 @@ __global__ __launch_bounds__(kMaxGrid) void paged_merge_kernel(AttnParams p, uin
     MergeDesc mine{};
     if (tid < n_descs) mine = p.descs[tid];
     const uint32_t items = mine.rows == 0 ? 0 : together(mine.last - tid + 1) ? (mine.rows + SL - 1) / SL : mine.rows;
-    uint32_t upto = items;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(upto, o, 64);
-        if ((int)lane >= o) upto += y;
-    }
+    uint32_t upto = sums_upto(items);
     if (lane == 63) s_wave[tid >> 6] = upto;
     __syncthreads();
     uint32_t total = 0;
