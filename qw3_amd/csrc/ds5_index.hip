@@ -166,7 +166,7 @@ uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* 
     for (uint32_t b = 0; b < n_seqs; b++) per_head += n[b] ? pb_seq_work(seq(b), group) : 0;
     const double total = per_head * n_kv_heads;
     if (total == 0) return 0;
-    const uint32_t n_wg = whole ? grid : pb_workgroups(total, group, n_kv_heads, grid);
+    const uint32_t n_wg = whole ? grid : pb_workgroups(total, 1.0 / group, n_kv_heads, 1.0 / n_kv_heads, grid);
     const double share = pb_inverse(n_wg);
     const double snap = pb_snap(total, share, group);
     double line = 0;

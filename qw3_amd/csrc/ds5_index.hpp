@@ -272,13 +272,16 @@ struct PbPlace {
 };
 DS5_HD PbPlace pb_locate(PbSeq s, uint32_t group, double inv_group, double y, double snap, double lead, bool whole) {
     const uint32_t nt = pb_tiles(s, group);
-    const double pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
-    double off;
-    uint32_t j = pb_divide(y, pair, off) * 2;
-    const double heavy = pb_tile_work(s, group, pb_tile_at(j, nt));
-    if (j + 1 < nt && off >= heavy) {
-        j++;
-        off -= heavy;
+    double off = y;
+    uint32_t j = 0;
+    if (nt > 1) {
+        const double pair = pb_tile_work(s, group, nt - 1) + pb_tile_work(s, group, 0);
+        j = pb_divide(y, pair, off) * 2;
+        const double heavy = pb_tile_work(s, group, pb_tile_at(j, nt));
+        if (j + 1 < nt && off >= heavy) {
+            j++;
+            off -= heavy;
+        }
     }
     const uint32_t tile = pb_tile_at(j, nt);
     const double w = pb_tile_work(s, group, tile), at = y - off;
@@ -308,10 +311,10 @@ DS5_HD double pb_lead(double work, double part, uint32_t group) {
 }
 // The workgroups that share a line of work: kPbPiece of a row's work each at least, and the same number
 // for each kv head where there are enough, so that no workgroup ends one head's tile to begin another's.
-DS5_HD uint32_t pb_workgroups(double work, uint32_t group, uint32_t heads, uint32_t grid) {
-    const double n = work * pb_inverse((double)group * kPbPiece);
+DS5_HD uint32_t pb_workgroups(double work, double inv_group, uint32_t heads, double inv_heads, uint32_t grid) {
+    const double n = work * inv_group * (1.0 / kPbPiece);
     const uint32_t all = n >= (double)grid ? grid : n < 1.0 ? 1 : (uint32_t)n;
-    return all > heads ? all / heads * heads : all;
+    return all > heads ? pb_over(all, inv_heads) * heads : all;
 }
 // Moves c on to the next tile that has rows; false where that is past the part that ends at `end`.
 // at_end: the part ends inside this tile, at position end.k. seq(b) gives sequence b.

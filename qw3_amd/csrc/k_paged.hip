@@ -189,7 +189,7 @@ struct MergeDesc {
 struct AttnParams {
     PagedAttentionLaunch a;
     uint32_t group;
-    double inv_group, inv_page;  // 1 / group, 1 / page_size
+    double inv_group, inv_page, inv_heads;  // 1 / group, 1 / page_size, 1 / n_kv_heads
     bool whole;        // no tile is cut
     float* part_o;     // [2 * workgroups, kRows, D]: slot 2 w the part that workgroup w continues, 2 w + 1 the one it begins
     float2* part_ml;   // [2 * workgroups, kRows]: reference and sum
@@ -675,7 +675,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         }
         const double total = per_head * bt.n_kv_heads;
         const uint32_t grid = gridDim.x;
-        const uint32_t n_wg = uniform(total == 0.0 ? 0 : p.whole ? grid : ds5idx::pb_workgroups(total, G, bt.n_kv_heads, grid));
+        const uint32_t n_wg = uniform(total == 0.0 ? 0 : p.whole ? grid : ds5idx::pb_workgroups(total, p.inv_group, bt.n_kv_heads, p.inv_heads, grid));
         // A full grid's consecutive parts go to one XCD (workgroup i runs on XCD i % 8), so that a
         // sequence's K and V come into few L2s.
         const uint32_t wg = n_wg + bt.n_kv_heads > grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
@@ -1198,6 +1198,7 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     p.group = b.n_q_heads / b.n_kv_heads;
     p.inv_group = 1.0 / p.group;
     p.inv_page = 1.0 / b.page_size;
+    p.inv_heads = 1.0 / b.n_kv_heads;
     const uint64_t rows = (uint64_t)b.n_tokens * p.group, tiles = rows / kRows + std::min<uint64_t>(b.n_seqs, b.n_tokens);
     // the work that the plan counts, at most: below 2^53
     if ((double)b.n_kv_heads * tiles * ((double)p.group * (5.0 * b.max_seq_len + ds5idx::kPbTileCost) + 5.0 * (rows + kRows)) >= 9007199254740992.0)
