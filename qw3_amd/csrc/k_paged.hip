@@ -181,8 +181,6 @@ constexpr uint32_t kWindow = 1024;  // groups of 16 positions whose place in the
 constexpr float kHead = 8.0f, kMove = 15.0f;
 
 struct MergeDesc {
-    uint32_t last;  // the tile's parts: this workgroup's head part, then workgroups w + 1 .. last
-    uint32_t rows;  // 0: nothing to merge
     uint32_t row0, kvh, token0;
 };
 
@@ -193,7 +191,11 @@ struct AttnParams {
     bool whole;        // no tile is cut
     float* part_o;     // [2 * workgroups, kRows, D]: slot 2 w the part that workgroup w continues, 2 w + 1 the one it begins
     float2* part_ml;   // [2 * workgroups, kRows]: reference and sum
-    MergeDesc* descs;  // [workgroups]
+    // [workgroups]: of the tile that the workgroup begins and does not end (0: none) its rows, and above them the
+    // last workgroup with a part of it: the parts are this one's head part, then those of w + 1 .. last. (In a word
+    // of its own, as every workgroup of the merge reads them all: 20 bytes each made it 17 us instead of 4.)
+    uint32_t* heads;
+    MergeDesc* descs;
 };
 
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
@@ -679,7 +681,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
         // A full grid's consecutive parts go to one XCD (workgroup i runs on XCD i % 8), so that a
         // sequence's K and V come into few L2s.
         const uint32_t wg = n_wg + bt.n_kv_heads > grid && grid % 8 == 0 ? blockIdx.x % 8 * (grid / 8) + blockIdx.x / 8 : blockIdx.x;
-        if (tid == 0 && p.descs) p.descs[wg].rows = 0;  // until it begins a tile that it does not end
+        if (tid == 0 && p.heads) p.heads[wg] = 0;  // until it begins a tile that it does not end
         if (wg >= n_wg) return;
         const double share = ds5idx::pb_inverse(n_wg);
         const double snap = ds5idx::pb_snap(total, share, G);
@@ -1052,8 +1054,10 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
             // the last workgroup with a part of the tile: the last cut that is not within `snap` of its end
             if (begins && !poison) {
                 const double share = ds5idx::pb_inverse(w.n_wg);
-                p.descs[wg] = MergeDesc{ds5idx::pb_last_cut(w.total, w.n_wg, share, tile_end - ds5idx::pb_snap(w.total, share, G)),
-                                        rows, row0, kvh, start};
+                const uint32_t last = ds5idx::pb_last_cut(w.total, w.n_wg, share, tile_end - ds5idx::pb_snap(w.total, share, G));
+                static_assert(kRows < 256 && kMaxGrid <= 1u << 24, "rows and workgroup in a word");
+                p.heads[wg] = rows | last << 8;
+                p.descs[wg] = MergeDesc{row0, kvh, start};
             }
             w.line = tile_end;
         }
@@ -1071,15 +1075,14 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
 template <int D>
 __global__ __launch_bounds__(kMaxGrid) void paged_merge_kernel(AttnParams p, uint32_t n_descs) {
     constexpr uint32_t CH = D / 4, SL = kMaxGrid / CH;
-    __shared__ uint32_t s_upto[kMaxGrid];  // items of the tiles up to and with this one
-    __shared__ uint32_t s_wave[kMaxGrid / 64], s_item;
+    __shared__ uint32_t s_wave[kMaxGrid / 64];
+    __shared__ uint32_t s_item[3];  // the item at hand: its head part's workgroup, its place among the tile's items, the tile's word
     __shared__ f32x4 s_o[SL][CH];
     __shared__ float2 s_ml[SL];
     const uint32_t tid = threadIdx.x, lane = tid & 63, G = p.group;
     auto together = [&](uint32_t parts) { return parts <= SL; };  // SL rows at once
-    MergeDesc mine{};
-    if (tid < n_descs) mine = p.descs[tid];
-    const uint32_t items = mine.rows == 0 ? 0 : together(mine.last - tid + 1) ? (mine.rows + SL - 1) / SL : mine.rows;
+    const uint32_t mine = tid < n_descs ? p.heads[tid] : 0, mine_rows = mine & 255;
+    const uint32_t items = mine == 0 ? 0 : together((mine >> 8) - tid + 1) ? (mine_rows + SL - 1) / SL : mine_rows;
     uint32_t upto = sums_upto(items);
     if (lane == 63) s_wave[tid >> 6] = upto;
     __syncthreads();
@@ -1089,15 +1092,17 @@ __global__ __launch_bounds__(kMaxGrid) void paged_merge_kernel(AttnParams p, uin
         if (w < tid >> 6) upto += s_wave[w];
         total += s_wave[w];
     }
-    s_upto[tid] = upto;
-    __syncthreads();
     const uint32_t c = tid % CH, sl = tid / CH;
     for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
-        if (item < upto && item >= upto - items) s_item = tid;  // one thread's
+        if (item < upto && item >= upto - items) {  // one thread's
+            s_item[0] = tid;
+            s_item[1] = item - (upto - items);
+            s_item[2] = mine;
+        }
         __syncthreads();
-        const uint32_t w = uniform(s_item);
+        const uint32_t w = uniform(s_item[0]), at = uniform(s_item[1]), head = uniform(s_item[2]);
         const MergeDesc d = p.descs[w];
-        const uint32_t n = d.last - w + 1, at = item - (w ? s_upto[w - 1] : 0);
+        const uint32_t n = (head >> 8) - w + 1;
         // parts first, first + step, ... of a row
         auto fold = [&](uint32_t row, uint32_t first, uint32_t step, float& M, float& L, f32x4& o) {
             constexpr int U = 8;
@@ -1128,15 +1133,15 @@ __global__ __launch_bounds__(kMaxGrid) void paged_merge_kernel(AttnParams p, uin
             }
         };
         auto write = [&](uint32_t row, f32x4 o, float L) {
-            const uint32_t packed = d.row0 + row;
-            *(f32x4*)(p.a.out + ((uint64_t)(d.token0 + packed / G) * p.a.batch.n_q_heads + d.kvh * G + packed % G) * D + 4 * c) =
+            const uint32_t packed = d.row0 + row, token = ds5idx::pb_over(packed, p.inv_group);
+            *(f32x4*)(p.a.out + ((uint64_t)(d.token0 + token) * p.a.batch.n_q_heads + d.kvh * G + (packed - token * G)) * D + 4 * c) =
                 o * (1.0f / L);
         };
         float M, L;
         f32x4 o;
         if (together(n)) {
             const uint32_t row = at * SL + sl;
-            if (row < d.rows) {
+            if (row < (head & 255)) {
                 fold(row, 0, 1, M, L, o);
                 write(row, o, L);
             }
@@ -1210,10 +1215,11 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     const dim3 grid((uint32_t)std::min<uint64_t>(most, cus)), block(kThreads);
     if (!p.whole) {
         static_assert(2ull * kMaxGrid * kRows * 128 * sizeof(float) <= kSplitBytesMax, "parts fit the context's buffer");
-        static_assert(2ull * kMaxGrid * kRows * sizeof(float2) + kMaxGrid * sizeof(MergeDesc) <= kSplitStateBytes, "and their state");
+        static_assert(2ull * kMaxGrid * kRows * sizeof(float2) + kMaxGrid * (sizeof(MergeDesc) + 4) <= kSplitStateBytes, "and their state");
         p.part_o = (float*)ctx->split_buf;
         p.part_ml = (float2*)((char*)ctx->split_buf + kSplitBytesMax);
-        p.descs = (MergeDesc*)(p.part_ml + 2ull * kMaxGrid * kRows);
+        p.heads = (uint32_t*)(p.part_ml + 2ull * kMaxGrid * kRows);
+        p.descs = (MergeDesc*)(p.heads + kMaxGrid);
     }
     const char* name = "paged_attention_kernel";
     if (b.head_dim == 128) {
