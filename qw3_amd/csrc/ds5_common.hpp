@@ -66,9 +66,9 @@ struct ds5_hip_ctx {
     size_t scratch_bytes = 0;
     bool use_scratch = false;
     // kSplitBytesMax + kSplitStateBytes for the partial results of an attention launch split over
-    // its keys (prefill, f32 caches, paged batches), allocated at init: whether a call splits then depends on its shape
-    // alone, captured or not, whatever ran before it. Null if there was no memory for it: such
-    // a context runs those launches unsplit.
+    // its keys (prefill, f32 caches, paged batches), allocated at init: whether a call splits then
+    // depends on its shape alone, captured or not, whatever ran before it. Null if there was no
+    // memory for it: such a context runs those launches unsplit.
     void* split_buf = nullptr;
     // Decode tuning: positions per split-K workgroup (0 = heuristic); paged
     // plan: workgroups per launch the plan aims at (0 = two per CU).

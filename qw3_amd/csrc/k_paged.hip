@@ -164,11 +164,11 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppen
 // are folded through LDS at the end. K and V come by direct-to-LDS loads, a block or three steps ahead.
 //
 // What bounds it. Long decode: memory; 32 sequences of 0.5 .. 16 K positions (4 kv heads of 128, 584 MB)
-// 114 us, 5.1 TB/s. Prompts: the matrix cores at the power that they may draw; 64 positions of 128 rows
+// 112 us, 5.2 TB/s. Prompts: the matrix cores at the power that they may draw; 64 positions of 128 rows
 // take 1.3 us with f16 q (48 products of 32 cycles a wavefront pair) and 1.5 with f32 q (64): 1.2 and 1.4
 // PFLOP/s issued, above a large library product's 1.14; leaving out the exponentials, the V reads or the
-// barriers changed neither. A prompt of 2048 69 us, 203 f32 tokens at 6000 88 + 8 merging. Small calls:
-// the chain of launch, plan, page table, K, V and output, 9 .. 14 us and 4 for the merge.
+// barriers changed neither. A prompt of 2048 68 us, 203 f32 tokens at 6000 87 + 7 merging. Small calls:
+// the chain of launch, plan, page table, K, V and output, 9 .. 13 us and 4 for the merge.
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 512, kWaves = 8;
 constexpr int kRows = ds5idx::kPbRows, kNarrow = ds5idx::kPbNarrow;
@@ -395,8 +395,8 @@ struct Attn {
         if constexpr (NB == 4)
             asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\t"
                          "global_load_lds_dwordx4 %1, %4 offset:1024\n\tglobal_load_lds_dwordx4 %2, %4 offset:2048\n\t"
-                         "global_load_lds_dwordx4 %3, %4 offset:3072" ::"v"(off), "v"(o1), "v"(o2), "v"(o3), "s"(base),
-                         "s"(uniform(lds))
+                         "global_load_lds_dwordx4 %3, %4 offset:%6" ::"v"(off), "v"(o1), "v"(o2), "v"(o3), "s"(base),
+                         "s"(uniform(lds)), "n"(3 * 1024)
                          : "m0", "memory");
         else
             asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\t"
@@ -496,12 +496,13 @@ struct Attn {
             }
     }
 
-    // One block of a run of them: its scores S (largest mx) stand already; the products of the next block's, Sn,
-    // (K at sk; after the last block whatever lies there, its scores dropped) go beside the weights of S, the products with V beside the other half of the
-    // weights and the next scores' maximum. load_k(), load_v(): later rows' loads, issued between products,
-    // where the wait for the load path to take them costs nothing. LDS reads run kAhead operands ahead of their products. The
-    // scheduling fences keep this order: a product occupies the matrix core for 32 cycles, in which the
-    // wavefront issues the VALU work beside it.
+    // One block of a run of them: its scores S (largest mx) stand already. The products of the next block's,
+    // Sn (K at k; after the last block whatever lies there, its scores dropped), go beside the weights of S,
+    // the products with V beside the other half of the weights and the next scores' maximum. load_k(),
+    // load_v(): later rows' loads, issued between products, where the wait for the load path to take them
+    // costs nothing. LDS reads run kAhead operands ahead of their products. The scheduling fences keep this
+    // order: a product occupies the matrix core for 32 cycles, in which the wavefront issues the VALU work
+    // beside it.
     template <class LoadK, class LoadV>
     __device__ __forceinline__ void step(f32x16& S, f32x16& Sn, float& mx, uint32_t k, uint32_t v, LoadK load_k, LoadV load_v) {
         constexpr int kAhead = 3, NV = 2 * DT, E0 = 8 / KS, E1 = 8 / DT;
@@ -1071,7 +1072,7 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
 // w + 1 .. last, folded in that order. 256 threads are D / 4 columns and 1024 / D slots: with few parts a
 // slot folds a row of its own, with many the slots share a row's parts and join through LDS. The
 // workgroups go along all tiles' rows (or groups of rows) evenly. 4 us where there is little (its launch),
-// 8 for the 17 MB of 256 parts of 128 rows of 128.
+// 7.5 for the 17 MB of 256 parts of 128 rows of 128.
 template <int D>
 __global__ __launch_bounds__(kMaxGrid) void paged_merge_kernel(AttnParams p, uint32_t n_descs) {
     constexpr uint32_t CH = D / 4, SL = kMaxGrid / CH;
@@ -1185,9 +1186,9 @@ int launch_paged_append(ds5_hip_ctx* ctx, const PagedAppendLaunch& a) {
 // Whether uncut tiles are the faster form, in the plan's units (4.7 ns), every sequence taken to have the
 // mean rows and the longest length: rounds of whole tiles, or even shares, in which a workgroup pays for a
 // second tile as a rule, and the merge with the parts' way through memory. Measured, us, cut and whole
-// (32 query and 4 kv heads of 128): one token 15.6 and 14.4 at 500 positions, 16.1 and 17.5 at 1000; 48
-// sequences' 29.1 and 18.5, 33.8 and 24.6, at 2000 43.5 and 39.7; six tokens 18.9 and 22.6, 20.3 and 31.7;
-// 48 sequences of six 37.4 and 26.3, 44.5 and 36.1; eight of 40 31.8 and 25.5, 42.0 and 35.1, 47.0 and 55.6.
+// (32 query and 4 kv heads of 128): one token 14.5 and 14.1 at 500 positions, 15.0 and 16.9 at 1000; 48
+// sequences' 27.1 and 17.3, 33.4 and 23.6, at 2000 42.0 and 37.6; six tokens 17.5 and 21.2, 18.8 and 30.3;
+// 48 sequences of six 34.7 and 24.3, 41.9 and 33.7; eight of 40 30.0 and 23.7, 39.5 and 33.1, 44.4 and 52.1.
 static bool whole_tiles_do(const PagedBatch& b, uint32_t group, uint32_t cus) {
     const double live = std::min(b.n_seqs, b.n_tokens), rows = std::ceil(b.n_tokens / live) * group;
     const bool wide = rows > kNarrow;
