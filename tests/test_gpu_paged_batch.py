@@ -68,6 +68,8 @@ ATTENTION = [  # ctx, new, hq, hkv, d, page
     ([40, 10, 9, 0], [0, 3, 0, 1], 16, 2, 64, 16),  # sequences without rows
     ([0] * 40 + [512] * 24, [1] * 40 + [2] * 24, 8, 8, 64, 16),
     ([3] * 130, [1, 2] * 65, 4, 2, 128, 16),  # more sequences than lanes
+    ([9000, 4000], [40, 1], 24, 3, 64, 16),   # three kv heads: 255 workgroups
+    ([2500, 0, 700], [700, 90, 1], 12, 6, 128, 80),
 ]
 
 
