@@ -205,15 +205,15 @@ DS5_HD uint32_t af_row_splits(uint32_t lim, uint32_t chunk) { return lim / chunk
 // tile in the order last, first, last but one, second, ... (a pair of them costs the same for
 // every pair), its positions. Workgroup w of n takes the part from w / n to (w + 1) / n of it.
 // Work is counted in half positions * group for the tiles of sequences of at most kPbNarrow rows
-// and in sixths for the others (64 positions measured 0.5 .. 0.7 us and 1.3 .. 1.5: 3.9 ns a unit),
+// and in fifths for the others (64 positions measured 0.5 .. 0.7 us and 1.3 .. 1.5: 4.7 ns a unit),
 // a tile's being its positions (taken as if every tile were full) and before them kPbTileCost for
-// beginning and ending it (9 .. 12 us). Six prompts and six single tokens take 111 us so and 113
-// with fifths and 2304, three and 37 with heads of 64 31.3 and 32.0. A workgroup whose part begins inside a tile, or ends there, pays that
+// beginning and ending it (9 .. 12 us). From caches in memory, two prompts among 22 single tokens
+// take 83 us so, 89 with sixths and 3200; six and six 120 and 124. A workgroup whose part begins inside a tile, or ends there, pays that
 // as every other does; what counts is the tiles that it begins after another, so the cost lies at
 // the tile's start, and cuts there fall on the start. A cut further on falls on a multiple of
 // kPbUnit positions, or on the tile's start or end where that is no further than `snap`.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 3200, kPbPiece = 384;
+constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 2304, kPbPiece = 384;
 
 struct PbSeq {
     uint32_t n, before;  // new tokens, and the tokens before them
@@ -227,7 +227,7 @@ struct PbCut {
 
 DS5_HD uint32_t pb_tiles(PbSeq s, uint32_t group) { return (s.n * group + kPbRows - 1) / kPbRows; }
 // Work as a double that holds an integer below 2^53 (the device multiplies 64-bit integers several times slower).
-DS5_HD double pb_weight(PbSeq s, uint32_t group) { return s.n * group > kPbNarrow ? 6.0 : 2.0; }
+DS5_HD double pb_weight(PbSeq s, uint32_t group) { return s.n * group > kPbNarrow ? 5.0 : 2.0; }
 DS5_HD double pb_tile_work(PbSeq s, uint32_t group, uint32_t tile) {
     return (double)group * kPbTileCost + pb_weight(s, group) * ((double)group * s.before + (double)kPbRows * (tile + 1));
 }

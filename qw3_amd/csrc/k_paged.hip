@@ -1183,19 +1183,19 @@ int launch_paged_append(ds5_hip_ctx* ctx, const PagedAppendLaunch& a) {
     return ds5_after_launch(ctx, name);
 }
 
-// Whether uncut tiles are the faster form, in the plan's units (3.9 ns), every sequence taken to have the
+// Whether uncut tiles are the faster form, in the plan's units (4.7 ns), every sequence taken to have the
 // mean rows and the longest length: rounds of whole tiles, or even shares, in which a workgroup pays for a
-// second tile as a rule, and the merge with the parts' way through memory. Measured, us, cut and whole
-// (32 query and 4 kv heads of 128): one token 14.5 and 14.1 at 500 positions, 15.0 and 16.9 at 1000; 48
-// sequences' 27.1 and 17.3, 33.4 and 23.6, at 2000 42.0 and 37.6; six tokens 17.5 and 21.2, 18.8 and 30.3;
-// 48 sequences of six 34.7 and 24.3, 41.9 and 33.7; eight of 40 30.0 and 23.7, 39.5 and 33.1, 44.4 and 52.1;
-// two prompts among 22 single tokens, up to 4000 positions, 69 and 65.
+// second tile as a rule, and the merge with the parts' way through memory. Measured with the caches in
+// memory (not in the chip's), us, cut and whole (32 query and 4 kv heads of 128): one token 15.8 and 14.8 at
+// 500 positions, 16.2 and 18.9 at 1000; 48 sequences' 37.7 and 29.3, 53.5 and 48.3, at 4000 145 and 137; six
+// tokens 18.2 and 22.0, 19.9 and 30.7; 48 sequences of six 42.2 and 33.4, 59.5 and 53.4; eight of 40 32.6
+// and 25.5, 43.7 and 35.0, at 2000 50.4 and 54.5.
 static bool whole_tiles_do(const PagedBatch& b, uint32_t group, uint32_t cus) {
     const double live = std::min(b.n_seqs, b.n_tokens), rows = std::ceil(b.n_tokens / live) * group;
     const bool wide = rows > kNarrow;
-    const double tile = ds5idx::kPbTileCost + (wide ? 6.0 : 2.0) * b.max_seq_len, tiles = b.n_kv_heads * live * std::ceil(rows / kRows);
+    const double tile = ds5idx::kPbTileCost + (wide ? 5.0 : 2.0) * b.max_seq_len, tiles = b.n_kv_heads * live * std::ceil(rows / kRows);
     const double n = std::min<double>(cus, std::max(1.0, tiles * tile / ds5idx::kPbPiece));
-    return std::ceil(tiles / cus) * tile <= tiles / n * tile + ds5idx::kPbTileCost + 1200.0 + (wide ? 2300.0 : 360.0) * n / cus;
+    return std::ceil(tiles / cus) * tile <= tiles / n * tile + ds5idx::kPbTileCost + 1350.0 + (wide ? 1300.0 : 300.0) * n / cus;
 }
 
 int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
@@ -1208,12 +1208,12 @@ int launch_paged_attention(ds5_hip_ctx* ctx, const PagedAttentionLaunch& a) {
     p.inv_heads = 1.0 / b.n_kv_heads;
     const uint64_t rows = (uint64_t)b.n_tokens * p.group, tiles = rows / kRows + std::min<uint64_t>(b.n_seqs, b.n_tokens);
     // the work that the plan counts, at most: below 2^53
-    if ((double)b.n_kv_heads * tiles * ((double)p.group * (6.0 * b.max_seq_len + ds5idx::kPbTileCost) + 6.0 * (rows + kRows)) >= 9007199254740992.0)
+    if ((double)b.n_kv_heads * tiles * ((double)p.group * (5.0 * b.max_seq_len + ds5idx::kPbTileCost) + 5.0 * (rows + kRows)) >= 9007199254740992.0)
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "paged_attention: batch too large");
     const uint32_t cus = std::min(kMaxGrid, ctx->cu_count > 0 ? (uint32_t)ctx->cu_count : kMaxGrid);
     p.whole = !ctx->split_buf || whole_tiles_do(b, p.group, cus);
     const uint64_t most =
-        b.n_kv_heads * tiles * (p.whole ? 1 : (6ull * b.max_seq_len + ds5idx::kPbTileCost) / ds5idx::kPbPiece + 1);
+        b.n_kv_heads * tiles * (p.whole ? 1 : (5ull * b.max_seq_len + ds5idx::kPbTileCost) / ds5idx::kPbPiece + 1);
     const dim3 grid((uint32_t)std::min<uint64_t>(most, cus)), block(kThreads);
     if (!p.whole) {
         static_assert(2ull * kMaxGrid * kRows * 128 * sizeof(float) <= kSplitBytesMax, "parts fit the context's buffer");
