@@ -46,6 +46,7 @@ struct LogprobsParams {
     uint64_t* keys;    // [n_rows, n_segs, top_n], descending, 0 past a segment's elements
 };
 
+constexpr uint32_t kLowest = 0x007fffffu;  // the order-preserving form of -inf
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t id) {
     const uint32_t u = __float_as_uint(x + 0.0f);  // -0 orders as +0
     const uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
@@ -200,8 +201,9 @@ __global__ __launch_bounds__(kThreads) void logprobs_part_kernel(LogprobsParams 
     if (p.top_n) {
         const uint64_t bound = find_bound(s_own, p.top_n);
         if (s_own[tid] >= bound) {
+            // (below the form of -inf, where fewer than top_n threads hold a finite logit, a prefix is no float's)
             const uint32_t o = (uint32_t)(bound >> 32);
-            const float least = bound == 1 ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+            const float least = o <= kLowest ? -INFINITY : __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 #pragma unroll
             for (int e = 0; e < PER; e++)
                 if (v[e] >= least && id_of(e) < p.vocab) {

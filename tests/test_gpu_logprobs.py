@@ -291,3 +291,38 @@ def test_two_graphs_share_the_workspaces(ctx, hip):
                 both()
     for _, graph, _, _ in calls:
         graph.destroy()
+
+
+def part_lengths(top, aligned):
+    """Lengths of a part of a row around those where top to 1.5 top of its threads hold a logit (four each where
+    the rows are 16-byte aligned)."""
+    k = 4 if aligned else 1
+    return sorted({n for n in (k * top - k, k * top - k + 1, k * top, k * (top + 1), k * (top + top // 2), k * (top + top // 2) + 1) if n >= top})
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("top", [2, 5, 20, 32])
+@pytest.mark.parametrize("segs", [0, 5])
+def test_few_finite_logits_in_a_part(ctx, hip, segs, top, aligned):
+    """A mask that leaves fewer finite logits than alternatives, in a short row and in the short last part of a long
+    one (2048 logits a part where rows of more than 8192 are few): every finite one is among the alternatives, then the lowest ids."""
+    for last in part_lengths(top, aligned):
+        V = 2048 * segs + last
+        g = np.random.default_rng([segs, top, last])
+        for left in sorted({1, top // 2, top - 1} - {0}):
+            x = np.full((3, V), -np.inf, np.float32)
+            for r in range(3):
+                x[r, 2048 * segs + g.choice(last, left, replace=False)] = g.standard_normal(left) * 3
+            if segs:
+                x[1, :2048 * segs] = g.standard_normal(2048 * segs) - 20  # less likely ones in the parts before
+                x[2, g.choice(2048 * segs, top, replace=False)] = 30 + g.standard_normal(top)  # and likelier ones
+            targets = x.argmax(1)
+            with np.errstate(invalid="ignore"):
+                want = reference(x, targets, top)
+            stride = V + (-V) % 4 if aligned else V + 1 - V % 2
+            got = run(ctx, hip, x, targets, top, stride)
+            assert np.array_equal(got[2], want[2]), (V, left)
+            t, finite = tolerance(x), np.isfinite(want[3])
+            assert np.array_equal(np.isfinite(got[3]), finite) and np.all(got[3][~finite] == -np.inf)
+            assert np.all(np.abs(got[3][finite] - want[3][finite]) <= t)
+            assert np.all(np.abs(got[0] - want[0]) <= t) and np.all(np.abs(got[1] - want[1]) <= 2 * t * (1 + want[1]))
