@@ -934,11 +934,14 @@ __global__ __launch_bounds__(kThreads) void paged_attention_kernel(AttnParams p)
                             run(i, Sa, Sb);
                             run(i + 1, Sb, Sa);
                         }
+                        // The last steps' loads ahead are still in flight past their barrier, into rows that O or
+                        // another window goes to: every wavefront waits for its own, then for the others.
                         wait_loads<0>();
+                        __syncthreads();
                     }
                     more = to < end;
                     if (more) {
-                        __syncthreads();  // everyone is done with the window
+                        if constexpr (narrow) __syncthreads();  // everyone is done with the window
                         window(to);
                         prime();
                     }

@@ -300,3 +300,13 @@ def test_append_attention_graph(ctx, hip):
     for a, b in zip(*outs):
         assert all(np.array_equal(x, y) for x, y in zip(a, b))
     assert not np.array_equal(outs[0][0][0], outs[0][3][0])
+
+
+@pytest.mark.parametrize("d,q_f16", [(128, False), (128, True), (64, False), (64, True)])
+def test_paged_attention_wide_tiles_again(ctx, hip, d, q_f16):
+    """Wide tiles of odd and even counts of 64-position steps, whole and cut, 40 times: right, and the same bits."""
+    c = Batch(22, [0, 1, 90, 150, 217, 281, 3000], [64, 130, 40, 41, 39, 300, 70], 16, 2, d, q_f16=q_f16)
+    check_attention(ctx, hip, c, q_f16)
+    want = run_attention(ctx, hip, c, q_f16)
+    for _ in range(20):
+        assert np.array_equal(run_attention(ctx, hip, c, q_f16).view(np.uint32), want.view(np.uint32))
