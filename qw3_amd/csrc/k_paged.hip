@@ -1128,7 +1128,7 @@ __global__ __launch_bounds__(kMaxGrid) void paged_merge_kernel(AttnParams p, uin
                 L *= f0, o *= f0;
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    if (i0 + u * step < n && ml[u].x != -INFINITY) {  // (a part of none of the row's positions holds nothing)
+                    if (i0 + u * step < n && ml[u].y != 0.0f) {  // (nothing: none of the row's positions; scores of NaN alone: -inf and NaN)
                         const float f = fast_exp2(ml[u].x - m);
                         L = __builtin_fmaf(ml[u].y, f, L);
                         o += v[u] * f;
@@ -1159,7 +1159,7 @@ __global__ __launch_bounds__(kMaxGrid) void paged_merge_kernel(AttnParams p, uin
                 for (uint32_t i = 0; i < SL; i++) mm = fmaxf(mm, s_ml[i].x);
                 f32x4 oo = {0.0f, 0.0f, 0.0f, 0.0f};
                 for (uint32_t i = 0; i < SL; i++) {
-                    if (s_ml[i].x == -INFINITY) continue;
+                    if (s_ml[i].y == 0.0f) continue;
                     const float f = fast_exp2(s_ml[i].x - mm);
                     ll += s_ml[i].y * f;
                     oo += s_o[i][c] * f;

@@ -310,3 +310,21 @@ def test_paged_attention_wide_tiles_again(ctx, hip, d, q_f16):
     want = run_attention(ctx, hip, c, q_f16)
     for _ in range(20):
         assert np.array_equal(run_attention(ctx, hip, c, q_f16).view(np.uint32), want.view(np.uint32))
+
+
+@pytest.mark.parametrize("new,d,q_f16", [(1, 128, False), (1, 64, True), (40, 128, True), (40, 64, False)])
+def test_paged_attention_keys_of_nan(ctx, hip, new, d, q_f16):
+    """NaN in every key of a span that ends, at one of the ends tried, where a part of the cut tile does: parts that hold
+    nothing else make the rows that attend them NaN all the same. The other kv head's rows, and another sequence's,
+    are as they were."""
+    c = Batch(21, [4000 - new, 50], [new, 1], 16, 2, d, q_f16=q_f16)
+    want, tol = c.attention()
+    tol = np.broadcast_to(tol, want.shape)
+    slots, kp = c.slots(0, 4000), c.kp.copy()
+    for end in [*range(64, 2048, 64), 4000]:
+        c.kp[1, slots[:end]] = np.nan
+        got = run_attention(ctx, hip, c, q_f16)
+        assert np.isnan(got[:new, 8:]).all(), end
+        err = np.abs(got - want)
+        assert np.all(err[:new, :8] <= tol[:new, :8]) and np.all(err[new:] <= tol[new:])
+        c.kp[:] = kp
