@@ -352,9 +352,10 @@ struct Attn {
     }
     __device__ __forceinline__ void form_q(const Query& q, float scale) {
         // fac stays above 0 (a negative scale goes into the row's sign), so that the largest product is
-        // the largest score and -inf stays -inf
+        // the largest score and -inf stays -inf; a scale of NaN stays NaN
         const bool minus = scale < 0.0f;
-        const float scale_log2 = fmaxf(fabsf(scale * kLog2e), 1e-37f);
+        auto positive = [](float x) { return x < 1e-37f ? 1e-37f : x; };
+        const float scale_log2 = positive(fabsf(scale * kLog2e));
         if constexpr (Q16) {
             fac = scale_log2;
 #pragma unroll
@@ -369,7 +370,7 @@ struct Attn {
                                        fmaxf(fmaxf(fabsf(q.x1[ks].x), fabsf(q.x1[ks].y)), fmaxf(fabsf(q.x1[ks].z), fabsf(q.x1[ks].w)))));
             big = swap32_op(big, OpMax{});
             const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 14 : 0;
-            fac = fmaxf(ldexpf(scale_log2, e), 1e-37f);
+            fac = positive(ldexpf(scale_log2, e));
             const float unit = minus ? -1.0f : 1.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {

@@ -328,3 +328,9 @@ def test_paged_attention_keys_of_nan(ctx, hip, new, d, q_f16):
         err = np.abs(got - want)
         assert np.all(err[:new, :8] <= tol[:new, :8]) and np.all(err[new:] <= tol[new:])
         c.kp[:] = kp
+
+
+@pytest.mark.parametrize("q_f16", [False, True])
+def test_paged_attention_scale_of_nan(ctx, hip, q_f16):
+    c = Batch(23, [5000, 90], [1, 40], 8, 2, 64, q_f16=q_f16)
+    assert np.isnan(run_attention(ctx, hip, c, q_f16, scale=float("nan"))).all()
