@@ -355,9 +355,8 @@ struct Attn {
         // the largest score and -inf stays -inf; a scale of NaN stays NaN
         const bool minus = scale < 0.0f;
         auto positive = [](float x) { return x < 1e-37f ? 1e-37f : x; };
-        const float scale_log2 = positive(fabsf(scale * kLog2e));
         if constexpr (Q16) {
-            fac = scale_log2;
+            fac = positive(fabsf(scale) * kLog2e);
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) qh[ks] = minus ? -q.h[ks] : q.h[ks];
         } else {
@@ -370,7 +369,7 @@ struct Attn {
                                        fmaxf(fmaxf(fabsf(q.x1[ks].x), fabsf(q.x1[ks].y)), fmaxf(fabsf(q.x1[ks].z), fabsf(q.x1[ks].w)))));
             big = swap32_op(big, OpMax{});
             const int e = big > 0.0f && big < INFINITY ? __builtin_amdgcn_frexp_expf(big) - 14 : 0;
-            fac = positive(ldexpf(scale_log2, e));
+            fac = positive(ldexpf(fabsf(scale), e) * kLog2e);
             const float unit = minus ? -1.0f : 1.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {

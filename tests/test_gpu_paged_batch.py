@@ -334,3 +334,11 @@ def test_paged_attention_keys_of_nan(ctx, hip, new, d, q_f16):
 def test_paged_attention_scale_of_nan(ctx, hip, q_f16):
     c = Batch(23, [5000, 90], [1, 40], 8, 2, 64, q_f16=q_f16)
     assert np.isnan(run_attention(ctx, hip, c, q_f16, scale=float("nan"))).all()
+
+
+def test_paged_attention_huge_q_tiny_scale(ctx, hip):
+    """A scale below the normal floats, of q near the largest: ordinary scores."""
+    c = Batch(24, [900, 200], [1, 40], 8, 2, 64)
+    c.q *= np.float32(3e37)
+    c.scale = float(np.float32(c.scale / 3e37))
+    check_attention(ctx, hip, c)
