@@ -543,7 +543,7 @@ int ds5_hip_paged_decode(ds5_hip_ctx* ctx, const ds5_paged_decode_args* args);
  * alone). q_out may be q itself when q_dtype is f32; other overlaps of the
  * outputs with the inputs are ShapeMismatch. A row that shows as NaN (see above)
  * does so in q_out, and its k and v are not appended. Two rows of one call must
- * not share a slot. At most 2^24 - 1 rows. */
+ * not share a slot. At most 2^24 - 1 rows and 2^31 - 1 sequences. */
 typedef struct ds5_paged_append_args {
     ds5_buf q;          /* optional f32 [n_tokens, n_q_heads, head_dim] */
     ds5_buf k;          /* f32 [n_tokens, n_kv_heads, head_dim] */

@@ -1077,6 +1077,8 @@ static int check_paged_batch(ds5_hip_ctx* ctx, const char* op, const PagedBatch&
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: max_seq_len exceeds max_pages * page_size", op);
     if (p.max_seq_len > INT32_MAX || p.n_tokens > INT32_MAX)  // what the i32 lengths and starts can say
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: max_seq_len or n_tokens above 2^31 - 1", op);
+    if (p.n_seqs > INT32_MAX)  // the append's search of starts adds to them in 32 bits
+        return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: more than 2^31 - 1 sequences", op);
     const uint64_t pool = size_of({p.n_kv_heads, p.n_pages, p.page_size, p.head_dim, 2});
     if (!covers(k_pool, pool) || !covers(v_pool, pool))
         return ds5_fail(ctx, DS5_SHAPE_MISMATCH, "%s: pool too small", op);

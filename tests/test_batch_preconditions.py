@@ -176,3 +176,11 @@ def test_score_refusals(hip):
     for tokens, targets, top in (([1, 2], [3], 0), ([1], [10], 0), ([1], [-1], 0), ([1], [1], 11), ([1], [1], -1)):
         with pytest.raises(ValueError):
             eng.score(tokens, np.array(targets), top)
+
+
+def test_more_sequences_than_the_rows_can_name(hip):
+    """A row's sequence is searched in 32 bits: 2^31 - 1 sequences at most, whatever the views hold."""
+    at = {n: hip.Buf((i + 1) << 44, 0, 1 << 43) for i, n in enumerate(("q", "k", "v", "q_norm", "k_norm", "q_out", "k_pool", "v_pool",
+                                                                       "page_table", "starts", "seq_lens"))}
+    for n, rc in ((2 ** 31 - 1, 3), (2 ** 31, 1), (2 ** 32 - 1, 1)):
+        assert rc_of(hip, "ds5_hip_paged_append", append(hip, **at, n_seqs=n)) == rc
