@@ -291,7 +291,7 @@ class Engine:
         tokens with theirs (arrays `logprobs`, `entropy` [n], `top_ids`, `top_logprobs` [n, top_n]).
         Only these come back to the host, not the logits (61 tokens of a 16384 vocabulary: 4 MB)."""
         n, vocab = len(tokens), self.cfg["vocab_size"]
-        if len(targets) != n:
+        if len(targets) != n or vocab > H.LOGPROBS_MAX_VOCAB:
             raise ValueError("BadShape")
         if top_n > min(vocab, H.LOGPROBS_MAX_TOP) or top_n < 0:
             raise ValueError("TopOutOfRange")

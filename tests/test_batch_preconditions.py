@@ -184,3 +184,14 @@ def test_more_sequences_than_the_rows_can_name(hip):
                                                                        "page_table", "starts", "seq_lens"))}
     for n, rc in ((2 ** 31 - 1, 3), (2 ** 31, 1), (2 ** 32 - 1, 1)):
         assert rc_of(hip, "ds5_hip_paged_append", append(hip, **at, n_seqs=n)) == rc
+
+
+def test_score_refuses_before_it_runs(hip):
+    """A vocabulary that the scores do not take is refused before the forward moves the engine on."""
+    from qw3_amd import engine as E
+    eng = E.Engine.__new__(E.Engine)
+    eng.cfg, eng.ctx, eng.scores, eng.max_batch, ran = dict(vocab_size=hip.LOGPROBS_MAX_VOCAB + 1), None, [None] * 5, 1, []
+    eng.forward = lambda *a, **k: ran.append(a)
+    with pytest.raises(ValueError):
+        eng.score([1], [1])
+    assert not ran
