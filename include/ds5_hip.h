@@ -576,11 +576,13 @@ int ds5_hip_paged_append(ds5_hip_ctx* ctx, const ds5_paged_append_args* args);
  * of its sequence attends positions 0 .. p (which the pool holds already, its own
  * among them); softmax in f32, out always f32. One call serves single tokens,
  * prompts and both mixed. f32 q enters the products with 22 significant bits,
- * f16 q (as ds5_hip_paged_append writes it) as it is; the softmax weights with 22
- * bits in either case. What a row does not attend never touches it, whatever the
- * pool holds there (infinities and NaN included). At most DS5_PAGED_MAX_SEQS
- * sequences; out must not overlap q or the pools. The same call gives the same
- * bits every time, captured or not. */
+ * f16 q (as ds5_hip_paged_append writes it) as it is; the softmax weights enter
+ * with 22 bits down to 2^-11 of the row's largest and below that to within 2^-33 of
+ * it, so that a long tail of n small weights is off by n 2^-33 of the values at most.
+ * What a row does not attend never touches it, whatever the pool holds there
+ * (infinities and NaN included); NaN in a key that it attends makes it NaN. At most
+ * DS5_PAGED_MAX_SEQS sequences; out must not overlap q or the pools. The same call
+ * gives the same bits every time, captured or not. */
 #define DS5_PAGED_MAX_SEQS 1024u
 typedef struct ds5_paged_attention_args {
     ds5_buf q;          /* q_dtype [n_tokens, n_q_heads, head_dim], normalised and rotated */

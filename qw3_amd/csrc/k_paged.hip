@@ -154,7 +154,7 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppen
 // One pass over the positions with the running reference and sums of a softmax. A kv head's query rows
 // (token * group + head) make tiles of 128, so that every K and V row is read once for 128 of them, on
 // v_mfma_f32_32x32x16_f16 with f32 accumulators. f32 accuracy from f16 operands: q (where it is f32) and
-// the weights are hi + lo pairs, two products each, 22 bits; K and V are f16 as they are.
+// the weights are hi + lo pairs, two products each, 22 bits (of the weights: see kHead); K and V are f16 as they are.
 //
 // How a batch is divided is known on the device only (starts, seq_lens): every workgroup works out its own
 // part of one line of all tiles' work, and parts of a tile are merged by a second kernel (ds5_index.hpp has
@@ -176,8 +176,10 @@ constexpr uint32_t kMaxSeqs = DS5_PAGED_MAX_SEQS;
 constexpr uint32_t kMaxGrid = 256;
 constexpr uint32_t kWindow = 1024;  // groups of 16 positions whose place in the pool is in LDS at a time
 // Weights are exp2(score - reference): the reference starts 2^8 below the row's maximum and moves
-// when a weight would pass 2^15, so that in f16 hi + lo a weight keeps its 22 bits down to 2^-22
-// of the largest and counts down to 2^-33 of it.
+// when a weight would pass 2^15. In f16 hi + lo a weight keeps its 22 bits down to 2^-3, 2^-11 of the
+// largest (lo is subnormal below), and is within 2^-25, 2^-33 of the largest, from there on: n positions
+// of such weights move a row by n 2^-33 of the values' size at most, 4e-6 for 2^15. (A reference nearer
+// to 2^15 would keep 22 bits further down and move with nearly every new maximum.)
 constexpr float kHead = 8.0f, kMove = 15.0f;
 
 struct MergeDesc {

@@ -342,3 +342,29 @@ def test_paged_attention_huge_q_tiny_scale(ctx, hip):
     c.q *= np.float32(3e37)
     c.scale = float(np.float32(c.scale / 3e37))
     check_attention(ctx, hip, c)
+
+
+@pytest.mark.parametrize("bits", [6, 11, 16, 22, 28, 34])
+@pytest.mark.parametrize("seqs,new", [(1, 1), (64, 1), (1, 40), (64, 20)])
+def test_paged_attention_flat_tail(ctx, hip, seqs, new, bits):
+    """One dominant position, of value 0, before 2^15 of equal weights 2^-bits of its own, of value 1: the weights' 22
+    bits, or 2^-33 of the dominant one, are what the sum over the tail may be off by. (64 sequences of the same
+    pages: whole tiles; one: cut.)"""
+    hq, hkv, d, L = 16, 4, 64, 2 ** 15
+    score = np.float32(bits * np.log(2.0))
+    q = np.zeros((seqs * new, hq, d), np.float32)
+    q[..., 0] = score
+    kp, vp = np.zeros((hkv, L, d), np.float16), np.ones((hkv, L, d), np.float16)
+    kp[:, 0, 0], vp[:, 0] = 8, 0
+    table = np.tile(np.arange(L // 16, dtype=np.int32), (seqs, 1))
+    out = ctx.createBuffer(q.nbytes)
+    hip.pagedAttention(ctx, hip.PagedAttentionArgs(
+        dev(ctx, q), dev(ctx, kp), dev(ctx, vp), dev(ctx, table), dev(ctx, np.arange(seqs + 1, dtype=np.int32) * np.int32(new)),
+        dev(ctx, np.full(seqs, L, np.int32)), out, hip.DTYPE_F32, seqs * new, seqs, hq, hkv, d, 16, L // 16, L // 16, L, 0.125))
+    got = ctx.to_numpy(out, np.float32, (seqs, new, hq * d))
+    tail = np.arange(L - new, L)[None, :, None].astype(np.float64) * np.exp(-np.float64(score))
+    want = tail / (1 + tail)
+    # relative: the score's 22 bits and its roundings in log2 units (3 half steps), the weight's 22 bits and its own
+    # rounding, and the sums', 16 positions a step; a weight's sum is of the unsplit weights, so that both count once
+    rel = 2.0 ** -22 * float(score) + bits * 3 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -23 + 2 * (L / 16 + 64) * 2.0 ** -24
+    assert np.all(np.abs(got - want) <= want * rel + L * 2.0 ** -33 / (1 + tail)), float(np.abs(got - want).max())
