@@ -575,8 +575,9 @@ int ds5_hip_paged_append(ds5_hip_ctx* ctx, const ds5_paged_append_args* args);
 /* Causal GQA attention of the batch's rows over the pool: row r at position p
  * of its sequence attends positions 0 .. p (which the pool holds already, its own
  * among them); softmax in f32, out always f32. One call serves single tokens,
- * prompts and both mixed. f32 q enters the products with 22 significant bits,
- * f16 q (as ds5_hip_paged_append writes it) as it is; the softmax weights enter
+ * prompts and both mixed. f32 q enters the products with 22 significant bits
+ * (elements below 2^-16 of their row's largest to within 2^-38 of that), f16 q
+ * (as ds5_hip_paged_append writes it) as it is; the softmax weights enter
  * with 22 bits down to 2^-11 of the row's largest and below that to within 2^-33 of
  * it, so that a long tail of n small weights is off by n 2^-33 of the values at most.
  * What a row does not attend never touches it, whatever the pool holds there

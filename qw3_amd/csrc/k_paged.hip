@@ -362,8 +362,9 @@ struct Attn {
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) qh[ks] = minus ? -q.h[ks] : q.h[ks];
         } else {
-            // the row times a power of two that brings its largest element to 2^13 .. 2^14: the
-            // operands then hold 22 bits of it whatever its size
+            // the row times a power of two that brings its largest element to 2^13 .. 2^14: whatever its
+            // size the operands hold 22 bits of elements down to 2^-2, 2^-16 of the largest, and smaller
+            // ones (lo is subnormal) to within 2^-25, 2^-38 of it
             float big = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)

@@ -368,3 +368,17 @@ def test_paged_attention_flat_tail(ctx, hip, seqs, new, bits):
     # rounding, and the sums', 16 positions a step; a weight's sum is of the unsplit weights, so that both count once
     rel = 2.0 ** -22 * float(score) + bits * 3 * 2.0 ** -24 + 2.0 ** -22 + 2.0 ** -23 + 2 * (L / 16 + 64) * 2.0 ** -24
     assert np.all(np.abs(got - want) <= want * rel + L * 2.0 ** -33 / (1 + tail)), float(np.abs(got - want).max())
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("bits", [8, 16, 20])
+def test_paged_attention_q_with_one_large_element(ctx, hip, new, bits):
+    """Elements of an f32 q beside one 2^bits as large, which meets zeros of K: 22 bits of each, or 2^-38 of the largest."""
+    c = Batch(25, [900], [new], 8, 2, 64)
+    c.q[..., 0] = np.ldexp(1.5, bits) * np.sign(c.q[..., 0])
+    c.kp[..., 0] = 0
+    want, tol = c.attention()
+    delta = c.scale * np.abs(np.nan_to_num(c.kp.astype(np.float64))).sum(-1).max() * 2.0 ** -38 * np.ldexp(1.5, bits)
+    got = run_attention(ctx, hip, c)
+    # a score off by delta moves its weight by as much of itself, and the weights' sum by as much again
+    assert np.all(np.abs(got - want) <= tol + 2 * delta * np.nanmax(np.abs(c.vp.astype(np.float64))))
