@@ -20,6 +20,9 @@ extern "C" {
  * direct-to-LDS loads. */
 uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* before, uint32_t group, uint32_t n_kv_heads,
                             uint32_t grid, int whole, uint32_t max, uint32_t* out);
+/* How far off, relative, the reciprocals' estimates are that ds5_index_pb_parts works from (0 at first; the
+ * device's at most 2^-22). */
+void ds5_index_pb_estimate(double error);
 void ds5_index_pb_loads(uint32_t head_dim, int v, uint32_t* off);
 
 #ifdef __cplusplus

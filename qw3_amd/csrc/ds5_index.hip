@@ -157,6 +157,7 @@ uint32_t ds5_index_af_store(uint32_t lim, uint32_t start, uint32_t chunk) {
 uint32_t ds5_index_af_row_splits(uint32_t lim, uint32_t chunk) { return ds5idx::af_row_splits(lim, chunk); }
 
 
+void ds5_index_pb_estimate(double error) { ds5idx::pb_estimate_error = error; }
 // The ragged batch's parts, workgroup by workgroup, as paged_attention_kernel walks them.
 uint32_t ds5_index_pb_parts(uint32_t n_seqs, const uint32_t* n, const uint32_t* before, uint32_t group, uint32_t n_kv_heads,
                             uint32_t grid, int whole, uint32_t max, uint32_t* out) {

@@ -243,14 +243,16 @@ DS5_HD PbTile pb_tile(PbSeq s, uint32_t group, double inv_group, uint32_t tile) 
     return PbTile{row0, end - row0, s.before + pb_over(end - 1, inv_group) + 1};
 }
 // 1 / d for d from 1 on, to 2^-44 or better: the device's estimate (to 2^-22) and one step of Newton's method.
-// (A division of doubles takes several times as long there, one of 64-bit integers longer still.)
+// (A division of doubles takes several times as long there, one of 64-bit integers longer still.) The host's, which
+// the tests walk the plan with, takes the step from an estimate as far off as they ask, another way for each d.
+inline double pb_estimate_error = 0.0;
 DS5_HD double pb_inverse(double d) {
 #if defined(__HIP_DEVICE_COMPILE__)
     const double r = __builtin_amdgcn_rcp(d);
-    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
 #else
-    return 1.0 / d;
+    const double r = (1.0 / d) * (1.0 + pb_estimate_error * sin(d));
 #endif
+    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
 }
 // x = q * d + r in integers, q below 2^32: the rounded quotient is at most one off.
 DS5_HD uint32_t pb_divide(double x, double d, double& r) {

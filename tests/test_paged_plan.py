@@ -107,3 +107,40 @@ def test_loads_cover_a_group_once(lib, d, v):
     slot, chunk, r = lds % (2 * d) // 16, off % (2 * d) // 16, lds // (2 * d)
     swz = {0: {128: r & 15, 64: (r >> 1) & 7}, 1: {128: 4 * (r & 3), 64: 4 * ((r >> 1) & 1)}}[v][d]
     assert np.array_equal(slot ^ chunk, swz)
+
+
+@pytest.fixture
+def estimate(lib):
+    """Sets the error of the reciprocals' estimates, and takes it back."""
+    lib.ds5_index_pb_estimate.argtypes, lib.ds5_index_pb_estimate.restype = [C.c_double], None
+    yield lib.ds5_index_pb_estimate
+    lib.ds5_index_pb_estimate(0.0)
+
+
+@pytest.mark.parametrize("bits", [22, 21])
+def test_plan_with_the_devices_reciprocals(lib, estimate, bits):
+    """The device's reciprocals are 2^-44 off at most, from estimates 2^-22 off: cuts may fall elsewhere, and every
+    position is still covered once, by parts that the merge finds."""
+    exact, moved = [], 0
+    g = np.random.default_rng(2)
+    batches = [(*b, grid, whole) for b in BATCHES for grid in (256, 255, 64, 7) for whole in (0, 1)]
+    for _ in range(300):
+        n = int(g.integers(1, 40))
+        new = (g.integers(0, 2, n) * np.exp(g.uniform(0, 6, n))).astype(int).tolist()
+        before = np.exp(g.uniform(0, 9, n)).astype(int).tolist()
+        batches.append((new, before, int(g.choice([1, 2, 3, 5, 8, 16, 130])), int(g.integers(1, 9)), int(g.choice([256, 200, 31])), int(g.integers(0, 2))))
+    estimate(0.0)
+    exact = [parts(lib, *b) for b in batches]
+    estimate(2.0 ** -bits)
+    for b, p in zip(batches, exact):
+        q = check(lib, *b)
+        moved += p.shape != q.shape or not np.array_equal(p, q)
+    print(f"{moved} of {len(batches)} plans moved")
+
+
+def test_the_estimates_error_reaches_the_plan(lib, estimate):
+    """(With an error that no device has: the cuts fall elsewhere.)"""
+    b = ([1] * 32, list(range(511, 16383, 496))[:32], 8, 4, 256, 0)
+    exact = parts(lib, *b)
+    estimate(2.0 ** -4)
+    assert not np.array_equal(parts(lib, *b), exact)
