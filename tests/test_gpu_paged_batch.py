@@ -382,3 +382,26 @@ def test_paged_attention_q_with_one_large_element(ctx, hip, new, bits):
     got = run_attention(ctx, hip, c)
     # a score off by delta moves its weight by as much of itself, and the weights' sum by as much again
     assert np.all(np.abs(got - want) <= tol + 2 * delta * np.nanmax(np.abs(c.vp.astype(np.float64))))
+
+
+def test_paged_append_refused_rows_write_nothing(ctx, hip):
+    """Neither pool changes but in the slots of the rows that are in range, with q and without."""
+    for with_q in (True, False):
+        c = Batch(26, [50, 20, 30], [2, 2, 17], 4, 2, 64, behind=1)
+        slots = c.slots(2, 32)[30:]         # positions 30 and 31 of sequence 2: the rows that are whole
+        c.seq_lens[0] = 1
+        c.table[1, 1] = c.n_pages           # the page of both rows of sequence 1
+        c.table[2, 2] = -1                  # positions 32 .. 46
+        q, k, v = (c.g.standard_normal((c.rows, h, c.d)).astype(np.float32) for h in (4, 2, 2))
+        none, kb, vb, qb = hip.Buf(), dev(ctx, c.kp), dev(ctx, c.vp), dev(ctx, q)
+        hip.pagedAppend(ctx, hip.PagedAppendArgs(qb if with_q else none, dev(ctx, k), dev(ctx, v), none, none, qb if with_q else none, kb, vb,
+                                                 dev(ctx, c.table), dev(ctx, c.starts), dev(ctx, c.seq_lens), *c.shape(hip, False), EPS, THETA, 1.0))
+        for b, was in ((kb, c.kp), (vb, c.vp)):
+            got = ctx.to_numpy(b, np.uint16, was.shape)
+            same = (got == was.view(np.uint16)).all(axis=(0, 2))
+            assert sorted(np.flatnonzero(~same)) == sorted(slots.tolist())
+        # f32: the rotation's roundings, 20 half steps of the pair at most; f16 its own half step
+        want = turned(k[4:6], None, [30, 31], THETA, EPS)
+        mag = np.hypot(k[4:6, :, :32], k[4:6, :, 32:])
+        got = ctx.to_numpy(kb, np.float16, c.kp.shape)[:, slots].transpose(1, 0, 2)
+        assert np.all(np.abs(got - want) <= np.concatenate([mag, mag], -1) * 20 * 2.0 ** -24 + np.abs(want) * 2.0 ** -11 + 2.0 ** -25)
