@@ -6,7 +6,8 @@ Shapes: the 32 q / 4 kv and 64 q / 4 kv heads of 128 of Qwen3-30B-A3B and Qwen3-
 vocabularies of the tests' size, of the benchmarks' models and generic ones.
 
 A batch (`op` append or attention) has `seqs` sequences with ctx_lo .. ctx_hi tokens cached; the first `chunks` of them
-bring new_lo .. new_hi new tokens, the others one. `own` false computes the operators in plain torch, true calls them.
+bring new_lo .. new_hi new tokens, the others one. `own` false computes the operators in plain torch, true calls them: on the
+context's stream, which torch's does not wait for, so that a synchronization goes before anything that reads what they wrote.
 """
 import math
 import random
@@ -110,8 +111,10 @@ def prepare(case, seed):
         # a text's own tokens are likelier than chance: half of them among the larger logits
         targets = torch.randint(0, V, (n,), generator=g, device=DEV)
         targets[::2] = x[::2, :V].argmax(1)
-        return dict(c=dict(c), x=x, targets=targets.to(torch.int32), logprobs=f(n), entropy=f(n),
-                    top_ids=torch.zeros(n, top, dtype=torch.int32, device=DEV), top_logprobs=f(n, top))
+        s = dict(c=dict(c), x=x, targets=targets.to(torch.int32), logprobs=f(n), entropy=f(n),
+                 top_ids=torch.zeros(n, top, dtype=torch.int32, device=DEV), top_logprobs=f(n, top))
+        torch.cuda.synchronize()  # the inputs are made on torch's stream, the calls run on the context's
+        return s
     ctx, new = _sizes(c)
     lens = [a + b for a, b in zip(ctx, new)]
     pages = [-(-n // c["page"]) for n in lens]
@@ -131,6 +134,7 @@ def prepare(case, seed):
                   k_norm=normal(d, std=0.02, mean=1.0), q_out=torch.zeros(T, hq, d, dtype=qt, device=DEV))
     else:
         s |= dict(q=normal(T, hq, d).to(qt), out=torch.zeros(T, hq * d, device=DEV))
+    torch.cuda.synchronize()
     return s
 
 
