@@ -205,13 +205,14 @@ DS5_HD uint32_t af_row_splits(uint32_t lim, uint32_t chunk) { return lim / chunk
 // tile in the order last, first, last but one, second, ... (a pair of them costs the same for
 // every pair), its positions. Workgroup w of n takes the part from w / n to (w + 1) / n of it.
 // Work is counted in half positions * group for the tiles of sequences of at most kPbNarrow rows
-// and in fifths for the others (64 positions measured 0.5 .. 0.7 us and 1.3 .. 1.5: 4.7 ns a unit),
-// a tile's being its positions (taken as if every tile were full) and before them kPbTileCost for
-// beginning and ending it (9 .. 12 us). From caches in memory, two prompts among 22 single tokens
-// take 83 us so, 89 with sixths and 3200; six and six 120 and 124. A workgroup whose part begins inside a tile, or ends there, pays that
-// as every other does; what counts is the tiles that it begins after another, so the cost lies at
-// the tile's start, and cuts there fall on the start. A cut further on falls on a multiple of
-// kPbUnit positions, or on the tile's start or end where that is no further than `snap`.
+// and in fifths for the others (64 positions of heads of 128 measured 0.5 .. 0.7 us and 1.3 .. 1.5: 4.7 ns
+// a unit), a tile's being its positions (taken as if every tile were full) and before them kPbTileCost
+// for beginning and ending it (9 .. 12 us). From caches in memory, two prompts among 22 single tokens
+// take 83 us so, 89 with sixths and 3200; six and six 120 and 124. A workgroup whose part begins inside
+// a tile, or ends there, pays that as every other does; what counts is the tiles that it begins after
+// another, so the cost lies at the tile's start, and cuts there fall on the start. A cut further on
+// falls on a multiple of kPbUnit positions, or on the tile's start or end where that is no further
+// than `snap`.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kPbRows = 128, kPbNarrow = 32, kPbUnit = 64, kPbTileCost = 2304, kPbPiece = 384;
 

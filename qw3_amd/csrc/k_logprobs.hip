@@ -12,8 +12,8 @@
 // state: m, S, C, A = sum (x_j - m) e_j, the target's logit where the segment holds it, and
 // the top_n largest keys in order. logprobs_join_kernel: a workgroup per row joins the
 // segments' states. Memory bound: the logits are read once; 512 rows of 65536 (134 MB) with five
-// alternatives take 27 us, 5.0 TB/s, and the join 5. One row of 65536 with 20 alternatives: two
-// launches of 5 us. (The join by the row's last segment, behind a fence and a counter, took longer:
+// alternatives take 28 us, 4.8 TB/s, and the join 5.5. One row of 65536 with 20 alternatives: two
+// launches of 6 and 5 us. (The join by the row's last segment, behind a fence and a counter, took longer:
 // 11.2 us instead of 10.2 for one row of 32768, 83 instead of 19 for 600 of 13578.)
 //
 // Selection by unique 64-bit keys (the logit in an order-preserving form above the complement of

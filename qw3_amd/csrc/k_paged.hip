@@ -164,11 +164,11 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(PagedAppen
 // are folded through LDS at the end. K and V come by direct-to-LDS loads, a block or three steps ahead.
 //
 // What bounds it. Long decode: memory; 32 sequences of 0.5 .. 16 K positions (4 kv heads of 128, 584 MB)
-// 112 us, 5.2 TB/s. Prompts: the matrix cores at the power that they may draw; 64 positions of 128 rows
+// 110 us, 5.3 TB/s. Prompts: the matrix cores at the power that they may draw; 64 positions of 128 rows
 // take 1.3 us with f16 q (48 products of 32 cycles a wavefront pair) and 1.5 with f32 q (64): 1.2 and 1.4
 // PFLOP/s issued, above a large library product's 1.14; leaving out the exponentials, the V reads or the
-// barriers changed neither. A prompt of 2048 68 us, 203 f32 tokens at 6000 87 + 7 merging. Small calls:
-// the chain of launch, plan, page table, K, V and output, 9 .. 13 us and 4 for the merge.
+// barriers changed neither. A prompt of 2048 65 us, 203 f32 tokens at 6000 86 + 8 merging. Small calls:
+// the chain of launch, plan, page table, q, K and V through LDS, and output, 9 .. 13 us and 4 for the merge.
 // ---------------------------------------------------------------------------
 constexpr int kThreads = 512, kWaves = 8;
 constexpr int kRows = ds5idx::kPbRows, kNarrow = ds5idx::kPbNarrow;
@@ -1190,7 +1190,9 @@ int launch_paged_append(ds5_hip_ctx* ctx, const PagedAppendLaunch& a) {
 }
 
 // Whether uncut tiles are the faster form, in the plan's units (4.7 ns), every sequence taken to have the
-// mean rows and the longest length: rounds of whole tiles, or even shares, in which a workgroup pays for a
+// mean rows and the longest length (the host knows no more, so that one long sequence among short ones whose
+// tiles come near a multiple of the CUs runs whole: 63 of 500 positions and one of 16384 151 us; 50 of 500 and
+// the long one, cut, 33): rounds of whole tiles, or even shares, in which a workgroup pays for a
 // second tile as a rule, and the merge with the parts' way through memory. Measured with the caches in
 // memory (not in the chip's), us, cut and whole (32 query and 4 kv heads of 128): one token 15.8 and 14.8 at
 // 500 positions, 16.2 and 18.9 at 1000; 48 sequences' 37.7 and 29.3, 53.5 and 48.3, at 4000 145 and 137; six
